@@ -26,7 +26,8 @@ EXPORTED = [
     "triattn_ipc_close", "triattn_peer_barrier", "triattn_peer_broadcast", "triattn_forward_chunked",
     "triattn_trimul_packed_bytes", "triattn_trimul_pack_weights", "triattn_trimul_workspace_bytes",
     "triattn_trimul_forward", "triattn_trimul_forward_addln", "triattn_forward_fused_tb",
-    "triattn_trimul_forward_addln_tb",
+    "triattn_trimul_forward_addln_tb", "triattn_layer_norm", "triattn_layer_norm_backward",
+    "triattn_layer_norm_backward_workspace_bytes", "triattn_dropout_add", "triattn_dropout_add_layer_norm",
 ]
 IPC_HANDLE_BYTES = 64
 
@@ -103,10 +104,19 @@ def lib() -> ctypes.CDLL:
         L.triattn_trimul_forward_addln.argtypes = [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]
         L.triattn_trimul_forward_addln_tb.argtypes = [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp,
                                                       _vp, _sz, _vp]
+        _d, _u = ctypes.c_double, ctypes.c_uint64
+        L.triattn_layer_norm.argtypes = [_vp, _i, _vp, _vp, _l, _vp, _vp, _i, _f, _vp, _i, _vp, _vp, _vp, _vp]
+        L.triattn_dropout_add.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _l, _i, _d, _u, _u, _vp, _vp, _i, _vp, _vp]
+        L.triattn_dropout_add_layer_norm.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _l, _i, _d, _u, _u, _vp, _vp, _vp,
+                                                     _i, _f, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]
+        L.triattn_layer_norm_backward_workspace_bytes.restype = _sz
+        L.triattn_layer_norm_backward_workspace_bytes.argtypes = [_l, _l]
+        L.triattn_layer_norm_backward.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _l, _vp, _i, _vp, _vp, _vp, _vp, _i,
+                                                  _d, _u, _u, _vp, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]
         for name in EXPORTED:
             if name not in ("triattn_version", "triattn_last_error_string", "triattn_packed_weights_bytes",
                             "triattn_workspace_bytes", "triattn_trimul_packed_bytes",
-                            "triattn_trimul_workspace_bytes"):
+                            "triattn_trimul_workspace_bytes", "triattn_layer_norm_backward_workspace_bytes"):
                 getattr(L, name).restype = ctypes.c_int
         _L = L
     return _L

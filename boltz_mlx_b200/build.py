@@ -14,8 +14,9 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtriattn.so"
-SOURCES = ["capi.cu", "kernels_f32.cu", "kernels_tc.cu", "noalloc.cu", "peer.cu", "trimul.cu"]
-HEADERS = ["sm100.cuh", "triattn_internal.cuh"]
+SOURCES = ["capi.cu", "kernels_f32.cu", "kernels_tc.cu", "noalloc.cu", "peer.cu", "trimul.cu",
+           "residual_capi.cu", "residual_fwd.cu", "residual_bwd.cu", "dropout_add.cu"]
+HEADERS = ["sm100.cuh", "triattn_internal.cuh", "residual.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -25,6 +26,7 @@ NVCC_FLAGS = [
     "-Xlinker", "-rpath,/usr/local/cuda/lib64",
     "--expt-relaxed-constexpr",
     "-lcublas",
+    "--threads", "0",  # the sources compile side by side
 ]
 
 

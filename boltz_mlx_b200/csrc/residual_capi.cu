@@ -1,0 +1,282 @@
+// extern "C" entry points of the residual path (declared in include/triattn.h): argument checks, strides
+// and mask positions, launches on the caller's stream.
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <utility>
+
+#include "residual.cuh"
+#include "triattn.h"
+
+using namespace triattn;
+
+namespace {
+
+int fail(int code, const char* what, const char* fmt, ...) {
+  char msg[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  return record_error(code, what, msg);
+}
+
+int finish(cudaError_t e, const char* what) {
+  return e == cudaSuccess ? TRIATTN_OK : record_error(TRIATTN_ECUDA, what, cudaGetErrorString(e));
+}
+
+bool known(int dtype) { return dtype == DT_F32 || dtype == DT_F16 || dtype == DT_BF16; }
+size_t bytes_of(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+
+// Shape of a call, and the widest access that all its tensors allow.
+struct Shape {
+  const char* what;
+  int64_t n[3];
+  int dim;
+  int64_t rows;
+  int vec;
+
+  int init(const char* name, const int64_t* shape, int64_t d, int64_t max_dim) {
+    what = name;
+    vec = 8;
+    if (!shape) return fail(TRIATTN_EINVAL, what, "shape is NULL");
+    if (d < 1) return fail(TRIATTN_EINVAL, what, "dim=%lld must be >= 1", (long long)d);
+    if (d > max_dim)
+      return fail(TRIATTN_EUNSUPPORTED, what, "dim=%lld above the supported %lld", (long long)d, (long long)max_dim);
+    rows = 1;
+    for (int k = 0; k < 3; ++k) {
+      n[k] = shape[k];
+      if (n[k] < 0) return fail(TRIATTN_EINVAL, what, "a negative size");
+      if (n[k] > 0x7fffffffLL) return fail(TRIATTN_EUNSUPPORTED, what, "2^31 rows or more");
+    }
+    for (int k = 0; k < 3; ++k) {
+      if (n[k] == 0) {
+        rows = 0;
+        break;
+      }
+      rows *= n[k];  // each factor and the product so far are below 2^31
+      if (rows > 0x7fffffffLL - (1 << 20)) {
+        // an empty axis further on still makes the call empty
+        for (int l = k + 1; l < 3; ++l)
+          if (n[l] == 0) rows = 0;
+        if (rows) return fail(TRIATTN_EUNSUPPORTED, what, "about 2^31 rows or more");
+        break;
+      }
+    }
+    dim = (int)d;
+    while (dim % vec) vec = vec == 8 ? 4 : 1;
+    return TRIATTN_OK;
+  }
+  RowMap map() const {
+    return RowMap{(uint32_t)rows, FastDiv::make((uint32_t)(n[1] ? n[1] : 1)), FastDiv::make((uint32_t)(n[2] ? n[2] : 1))};
+  }
+  // A tensor of this shape: its strides (NULL = dense), and what they and its address allow.  `written`:
+  // no two rows may share memory.
+  int tensor(const char* name, const void* p, int dtype, const int64_t* strides, Strides3* out, bool written) {
+    const size_t es = bytes_of(dtype);
+    if (!p) return fail(TRIATTN_EINVAL, what, "%s is NULL", name);
+    if (reinterpret_cast<uintptr_t>(p) % es) return fail(TRIATTN_EINVAL, what, "%s is not aligned to its elements", name);
+    const int64_t dense[3] = {n[1] * n[2] * dim, n[2] * dim, dim};
+    Strides3 s;
+    s.dense = true;
+    for (int k = 0; k < 3; ++k) {
+      s.s[k] = strides ? strides[k] : dense[k];
+      if (s.s[k] < 0) return fail(TRIATTN_EINVAL, what, "%s: negative stride", name);
+      if (n[k] > 1 && s.s[k] != dense[k]) s.dense = false;
+    }
+    if (written && !s.dense) {  // from the smallest stride up, each must clear what lies below it
+      int order[3] = {0, 1, 2};
+      for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2 - i; ++j)
+          if (s.s[order[j]] > s.s[order[j + 1]]) std::swap(order[j], order[j + 1]);
+      int64_t extent = dim;
+      for (int k : order) {
+        if (n[k] <= 1) continue;
+        if (s.s[k] < extent) return fail(TRIATTN_EINVAL, what, "%s: rows overlap", name);
+        extent += s.s[k] * (n[k] - 1);
+      }
+    }
+    // Dense rows need no check of the leading strides; others must allow the access at every row start.
+    while (vec > 1) {
+      bool ok = reinterpret_cast<uintptr_t>(p) % (vec * es < 16 ? vec * es : 16) == 0;
+      for (int k = 0; k < 3; ++k) ok = ok && (n[k] <= 1 || s.s[k] % vec == 0);
+      if (ok) break;
+      vec = vec == 8 ? 4 : 1;
+    }
+    *out = s;
+    return TRIATTN_OK;
+  }
+  // `share`: bit k = axis k (3: the channels) shares one draw
+  int dropout(int share, double p, uint64_t seed, uint64_t offset, const uint64_t* state, Dropout* out) const {
+    if (!(p >= 0.0 && p <= 1.0)) return fail(TRIATTN_EINVAL, what, "p=%g must lie in [0, 1]", p);
+    if (share < 0 || share > 15) return fail(TRIATTN_EINVAL, what, "share=%d is not a set of the axes 0..3", share);
+    if (reinterpret_cast<uintptr_t>(state) % 8) return fail(TRIATTN_EINVAL, what, "rng_state must be 8-byte aligned");
+    Dropout d{};
+    const uint64_t threshold = (uint64_t)(p * 4294967296.0 + 0.5);  // a word below it is dropped
+    d.on = threshold > 0;
+    d.drop_max = d.on ? (uint32_t)(threshold - 1) : 0;
+    d.scale = !d.on ? 1.0f : p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
+    d.seed = seed;
+    d.offset = offset;
+    d.state = state;
+    d.per_channel = share >> 3 & 1 ? 0 : 1;
+    int64_t m = d.per_channel ? dim : 1;
+    for (int k = 2; k >= 0; --k) {
+      d.m[k] = share >> k & 1 ? 0 : m;
+      if (!(share >> k & 1)) m *= n[k];
+    }
+    *out = d;
+    return TRIATTN_OK;
+  }
+};
+
+// The type pairs that the kernels are built for: an fp32 stream with an fp32 or 16-bit result, or one
+// 16-bit type throughout; y in the stream's type or in the result's.
+int check_types(const char* what, int z, int y, int out) {
+  if (!known(z) || !known(y) || !known(out)) return fail(TRIATTN_EUNSUPPORTED, what, "dtype %d, %d, %d", z, y, out);
+  const bool ok = z == DT_F32 ? (y == DT_F32 || y == out) : (y == z && out == z);
+  return ok ? TRIATTN_OK : fail(TRIATTN_EUNSUPPORTED, what, "type combination %d, %d -> %d", z, y, out);
+}
+
+int check_params(const char* what, const void* w, const void* b, int dtype, float eps) {
+  if (!known(dtype)) return fail(TRIATTN_EUNSUPPORTED, what, "parameter dtype %d", dtype);
+  const size_t es = bytes_of(dtype);
+  if (reinterpret_cast<uintptr_t>(w) % es || reinterpret_cast<uintptr_t>(b) % es)
+    return fail(TRIATTN_EINVAL, what, "a parameter is not aligned to its elements");
+  if (!(eps >= 0.0f) || std::isinf(eps)) return fail(TRIATTN_EINVAL, what, "eps=%g must be finite and >= 0", (double)eps);
+  return TRIATTN_OK;
+}
+
+int check_stats(const char* what, const float* mean, const float* rstd) {
+  if (reinterpret_cast<uintptr_t>(mean) % 4 || reinterpret_cast<uintptr_t>(rstd) % 4)
+    return fail(TRIATTN_EINVAL, what, "mean / rstd are not aligned to their elements");
+  return TRIATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int triattn_layer_norm(const void* x, int x_dtype, const int64_t* x_strides, const int64_t* shape, int64_t dim,
+                       const void* weight, const void* bias, int param_dtype, float eps, void* out, int out_dtype,
+                       const int64_t* out_strides, float* mean, float* rstd, void* stream) {
+  const char* what = "layer_norm";
+  Shape s;
+  if (int r = s.init(what, shape, dim, RES_MAX_DIM)) return r;
+  if (int r = check_types(what, x_dtype, x_dtype, out_dtype)) return r;
+  if (int r = check_params(what, weight, bias, param_dtype, eps)) return r;
+  if (int r = check_stats(what, mean, rstd)) return r;
+  if (s.rows == 0) return TRIATTN_OK;
+  NormFwdArgs a{};
+  if (int r = s.tensor("x", x, x_dtype, x_strides, &a.zs, false)) return r;
+  if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
+  a.z = x; a.out = out; a.map = s.map(); a.dim = s.dim;
+  a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
+  a.mean = mean; a.rstd = rstd;
+  return finish(launch_norm_fwd(a, x_dtype, x_dtype, out_dtype, s.vec, static_cast<cudaStream_t>(stream)), what);
+}
+
+int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, const void* y, int y_dtype,
+                        const int64_t* y_strides, const int64_t* shape, int64_t dim, int share, double p, uint64_t seed,
+                        uint64_t offset, const uint64_t* rng_state, void* out, int out_dtype,
+                        const int64_t* out_strides, void* stream) {
+  const char* what = "dropout_add";
+  Shape s;
+  DropoutAddArgs a{};
+  if (int r = s.init(what, shape, dim, 1 << 30)) return r;
+  if (!known(y_dtype) || !known(out_dtype) || (z && z_dtype != out_dtype))
+    return fail(TRIATTN_EUNSUPPORTED, what, "type combination %d, %d -> %d", z ? z_dtype : -1, y_dtype, out_dtype);
+  if (z ? (out_dtype != DT_F32 && y_dtype != out_dtype) : (y_dtype != DT_F32 && y_dtype != out_dtype))
+    return fail(TRIATTN_EUNSUPPORTED, what, "type combination %d, %d -> %d", z ? z_dtype : -1, y_dtype, out_dtype);
+  if (int r = s.dropout(share, p, seed, offset, rng_state, &a.drop)) return r;
+  if (s.rows == 0) return TRIATTN_OK;
+  if (z)
+    if (int r = s.tensor("z", z, z_dtype, z_strides, &a.zs, false)) return r;
+  if (int r = s.tensor("y", y, y_dtype, y_strides, &a.ys, false)) return r;
+  if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
+  a.z = z; a.y = y; a.out = out; a.map = s.map(); a.dim = s.dim;
+  a.in_place = z == out;
+  return finish(launch_dropout_add(a, z_dtype, y_dtype, out_dtype, s.vec, static_cast<cudaStream_t>(stream)), what);
+}
+
+int triattn_dropout_add_layer_norm(const void* z, int z_dtype, const int64_t* z_strides, const void* y, int y_dtype,
+                                   const int64_t* y_strides, const int64_t* shape, int64_t dim, int share, double p,
+                                   uint64_t seed, uint64_t offset, const uint64_t* rng_state, const void* weight,
+                                   const void* bias, int param_dtype, float eps, void* sum, const int64_t* sum_strides,
+                                   void* out, int out_dtype, const int64_t* out_strides, float* mean, float* rstd,
+                                   void* stream) {
+  const char* what = "dropout_add_layer_norm";
+  Shape s;
+  NormFwdArgs a{};
+  if (int r = s.init(what, shape, dim, RES_MAX_DIM)) return r;
+  if (int r = check_types(what, z_dtype, y_dtype, out_dtype)) return r;
+  if (int r = check_params(what, weight, bias, param_dtype, eps)) return r;
+  if (int r = check_stats(what, mean, rstd)) return r;
+  if (int r = s.dropout(share, p, seed, offset, rng_state, &a.drop)) return r;
+  if (s.rows == 0) return TRIATTN_OK;
+  if (int r = s.tensor("z", z, z_dtype, z_strides, &a.zs, false)) return r;
+  if (int r = s.tensor("y", y, y_dtype, y_strides, &a.ys, false)) return r;
+  if (int r = s.tensor("sum", sum, z_dtype, sum_strides, &a.ss, true)) return r;
+  if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
+  a.z = z; a.y = y; a.sum = sum; a.out = out; a.map = s.map(); a.dim = s.dim;
+  a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
+  a.mean = mean; a.rstd = rstd;
+  return finish(launch_norm_fwd(a, z_dtype, y_dtype, out_dtype, s.vec, static_cast<cudaStream_t>(stream)), what);
+}
+
+size_t triattn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim) {
+  if (rows < 1 || dim < 1 || dim > RES_MAX_DIM) return 0;
+  const int64_t ctas = norm_bwd_max_ctas();  // a CTA has one row at least
+  return (size_t)(rows < ctas ? rows : ctas) * 2 * (size_t)dim * sizeof(float);
+}
+
+int triattn_layer_norm_backward(const void* dout, int dout_dtype, const int64_t* dout_strides, const void* x, int x_dtype,
+                                const int64_t* x_strides, const int64_t* shape, int64_t dim, const void* weight,
+                                int param_dtype, const float* mean, const float* rstd, const void* dsum,
+                                const int64_t* dsum_strides, int share, double p, uint64_t seed, uint64_t offset,
+                                const uint64_t* rng_state, void* dx, void* dy, int y_dtype, void* dweight, void* dbias,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "layer_norm_backward";
+  Shape s;
+  NormBwdArgs a{};
+  Strides3 dense;
+  if (int r = s.init(what, shape, dim, RES_MAX_DIM)) return r;
+  if (!dy) y_dtype = x_dtype;
+  if (int r = check_types(what, x_dtype, y_dtype, dout_dtype)) return r;
+  if (int r = check_params(what, weight, dweight, param_dtype, 0.0f)) return r;
+  if (int r = check_params(what, weight, dbias, param_dtype, 0.0f)) return r;
+  if (int r = s.dropout(share, p, seed, offset, rng_state, &a.drop)) return r;
+  if (s.rows && (dweight || dbias)) {
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)
+      return fail(TRIATTN_EINVAL, what, "dweight / dbias need a 16-byte aligned workspace");
+    const size_t need = triattn_layer_norm_backward_workspace_bytes(s.rows, dim);
+    if (workspace_bytes < need) return fail(TRIATTN_ENOSPACE, what, "workspace %zu bytes < %zu needed", workspace_bytes, need);
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (s.rows == 0) {  // empty sums
+    const size_t n = (size_t)dim * bytes_of(param_dtype);
+    if (dweight)
+      if (int r = finish(cudaMemsetAsync(dweight, 0, n, st), what)) return r;
+    if (dbias)
+      if (int r = finish(cudaMemsetAsync(dbias, 0, n, st), what)) return r;
+    return TRIATTN_OK;
+  }
+  if (!mean || !rstd) return fail(TRIATTN_EINVAL, what, "mean / rstd are NULL");
+  if (int r = check_stats(what, mean, rstd)) return r;
+  if (int r = s.tensor("dout", dout, dout_dtype, dout_strides, &a.dos, false)) return r;
+  if (int r = s.tensor("x", x, x_dtype, x_strides, &a.xs, false)) return r;
+  if (dsum)
+    if (int r = s.tensor("dsum", dsum, x_dtype, dsum_strides, &a.dss, false)) return r;
+  if (dx)
+    if (int r = s.tensor("dx", dx, x_dtype, nullptr, &dense, true)) return r;
+  if (dy)
+    if (int r = s.tensor("dy", dy, y_dtype, nullptr, &dense, true)) return r;
+  if (!dx && !dy && !dweight && !dbias) return TRIATTN_OK;
+  a.dout = dout; a.x = x; a.ds = dsum; a.map = s.map(); a.dim = s.dim;
+  a.weight = weight; a.param_dtype = param_dtype; a.mean = mean; a.rstd = rstd;
+  a.dx = dx; a.dy = dy; a.dweight = dweight; a.dbias = dbias;
+  a.partial = dweight || dbias ? static_cast<float*>(workspace) : nullptr;
+  return finish(launch_norm_bwd(a, x_dtype, y_dtype, dout_dtype, s.vec, st), what);
+}
+
+}  // extern "C"

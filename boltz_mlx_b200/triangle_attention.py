@@ -29,6 +29,7 @@ import warnings
 
 from . import _lib
 from .layout import workspace_bytes
+from .residual import PairDropout, dropout_add, dropout_add_layer_norm, layer_norm
 
 
 @contextlib.contextmanager
@@ -227,8 +228,28 @@ class TriangleAttention(nn.Module):
             return self._run(x, mask, False, None, chunk_size)
         return self._run_fused(x, mask, xn, add_residual=False, keep_t=keep_t)[0]
 
+    def norm_input(self, z: torch.Tensor) -> torch.Tensor:
+        """This module's LayerNorm of z in its 16-bit type and attention orientation (for the ending node read
+        through the transposed view): the `xn` that forward and f16_addln take."""
+        dtype = _lib.dtype_code(self.precision)
+        if dtype == _lib.F32:
+            raise _lib.TriAttnUnsupported(_lib.EUNSUPPORTED, "xn belongs to the 16-bit path (precision fp16 or bf16)")
+        if z.dim() != 4 or z.shape[3] != self.c_in:
+            raise ValueError(f"z must be [B, N, N, {self.c_in}], got {tuple(z.shape)}")
+        ln = self.layer_norm
+        with torch.no_grad():
+            return layer_norm(z if self.starting else z.transpose(1, 2), ln.weight, ln.bias, ln.eps,
+                              torch.bfloat16 if dtype == _lib.BF16 else torch.float16)
+
+    def _draw_axes(self, dropout: PairDropout):
+        """The axes of [B, N, N, C] that share one draw: one draw per row (starting node) or per column."""
+        if dropout.share is not None:
+            return dropout.share
+        return (2, 3) if self.starting else (1, 3)
+
     def f16_addln(self, z: torch.Tensor, mask: Optional[torch.Tensor], xn: Optional[torch.Tensor], ln_next,
-                  trans_out: bool = False, tb: Optional[torch.Tensor] = None, w_tb: Optional[torch.Tensor] = None):
+                  trans_out: bool = False, tb: Optional[torch.Tensor] = None, w_tb: Optional[torch.Tensor] = None,
+                  dropout: Optional[PairDropout] = None):
         """(z + self(z), ln_next(z + self(z)) 16-bit [transposed with trans_out][, next tri bias]) as the
         reference's f16_addln (attention.py:170-190, kernels_nax3.linear_addln): the layer from
         xn = this module's LayerNorm output (ending node: already transposed), then the output projection,
@@ -239,7 +260,17 @@ class TriangleAttention(nn.Module):
         instead of its own LN . w_b dot (attention.py:128-147).  `w_tb` [H, c_in] (the next triangle
         attention's tb_weight16()): also return that module's tri bias, computed in the output kernel's
         epilogue from the rounded 16-bit LayerNorm rows (fp32 sums, one rounding to fp16), as
-        [B, H, Q, K] in ln_out's layout (the reference's PAIRTB, kernels_nax3.py:104-143)."""
+        [B, H, Q, K] in ln_out's layout (the reference's PAIRTB, kernels_nax3.py:104-143).  `dropout`: a training
+        step's dropout of the update, drawn in the pass that adds it and norms the sum (no w_tb then)."""
+        if dropout is not None:
+            if w_tb is not None:
+                raise _lib.TriAttnUnsupported(_lib.EUNSUPPORTED, "w_tb with dropout")
+            y = self._run_fused(z, mask, xn, add_residual=False, keep_t=False, tb=tb)[0]
+            with torch.no_grad():
+                return dropout_add_layer_norm(
+                    z.float(), y, ln_next.weight, ln_next.bias, dropout.p, dropout.seed, dropout.offset,
+                    share=self._draw_axes(dropout), eps=ln_next.eps, trans_out=trans_out,
+                    out_dtype=torch.bfloat16 if _lib.dtype_code(self.precision) == _lib.BF16 else torch.float16)
         z_new, ln_out, tb_next = self._run_fused(z, mask, xn, add_residual=True, keep_t=False, ln_next=ln_next,
                                                  trans_out=trans_out, tb=tb, w_tb=w_tb)
         if w_tb is None:
@@ -308,11 +339,19 @@ class TriangleAttention(nn.Module):
         return out, ln_out, tb_next
 
     def forward_residual(self, z: torch.Tensor, mask: Optional[torch.Tensor] = None, *,
-                         inplace: bool = False, chunk_size: Optional[int] = None) -> torch.Tensor:
-        """z + self(z) in one pass (the pairformer's residual update, pairformer.py:86-87)."""
+                         inplace: bool = False, chunk_size: Optional[int] = None,
+                         dropout: Optional[PairDropout] = None) -> torch.Tensor:
+        """z + self(z) in one pass (the pairformer's residual update, pairformer.py:86-87).  `dropout`: a training
+        step's dropout of the update (also in its passes without gradients): z + dropout(self(z))."""
         zc = z.contiguous()
-        out = zc if (inplace and zc is z and z.dtype == torch.float32) else None
-        return self._run(zc, mask, True, out, chunk_size)
+        own = inplace and zc is z and z.dtype == torch.float32
+        if dropout is not None:
+            y = self._run(zc, mask, False, None, chunk_size)
+            with torch.no_grad():
+                r = dropout_add(zc.detach().float(), y, dropout.p, dropout.seed, dropout.offset,
+                                share=self._draw_axes(dropout), inplace=own)
+            return zc if own else r
+        return self._run(zc, mask, True, zc if own else None, chunk_size)
 
 
 TriangleAttentionStartingNode = TriangleAttention

@@ -22,6 +22,7 @@ import torch
 from torch import nn
 
 from . import _lib
+from .residual import PairDropout, dropout_add, dropout_add_layer_norm
 from .triangle_attention import Workspace
 
 
@@ -93,21 +94,29 @@ class _TriangleMultiplication(nn.Module):
         return self._run(x, mask, False, None)
 
     def forward_residual(self, z: torch.Tensor, mask: Optional[torch.Tensor] = None, *,
-                         inplace: bool = False) -> torch.Tensor:
-        """z + self(z) in one pass (the pairformer's residual update)."""
+                         inplace: bool = False, dropout: Optional[PairDropout] = None) -> torch.Tensor:
+        """z + self(z) in one pass (the pairformer's residual update).  `dropout`: a training step's dropout of
+        the update, one draw per row by default: z + dropout(self(z))."""
         zc = z.contiguous()
-        out = zc if (inplace and zc is z and z.dtype == torch.float32) else None
-        return self._run(zc, mask, True, out)
+        own = inplace and zc is z and z.dtype == torch.float32
+        if dropout is not None:
+            y = self._run(zc, mask, False, None)
+            with torch.no_grad():
+                r = dropout_add(zc.detach().float(), y, dropout.p, dropout.seed, dropout.offset,
+                                share=(2, 3) if dropout.share is None else dropout.share, inplace=own)
+            return zc if own else r
+        return self._run(zc, mask, True, zc if own else None)
 
     def f16_addln(self, z: torch.Tensor, mask: Optional[torch.Tensor], xn: Optional[torch.Tensor], ln_next,
-                  w_tb: Optional[torch.Tensor] = None):
+                  w_tb: Optional[torch.Tensor] = None, dropout: Optional[PairDropout] = None):
         """(z + self(z), ln_next(z + self(z)) 16-bit[, next tri bias]) as the reference's f16_addln
         (triangular_mult.py:93-115): the output gate, the residual add and the next module's LayerNorm in
         the tail kernel.  16-bit precisions only.  `xn` (norm_in(z), precomputed) is accepted and
         recomputed from z.  `w_tb` [H, 128] (the next triangle attention's tb_weight16()): also return
         that module's tri bias, computed in the tail kernel's epilogue from the rounded 16-bit LayerNorm
         rows (fp32 sums, one rounding to fp16), as [B, H, N, N] (the reference's PAIRTB,
-        kernels_nax3.py:104-143)."""
+        kernels_nax3.py:104-143).  `dropout`: a training step's dropout of the update, drawn in the pass that
+        adds it and norms the sum (no w_tb then)."""
         del xn
         if not z.is_cuda:
             raise RuntimeError("TriangleMultiplication (B200) needs CUDA tensors; there is no CPU path")
@@ -117,6 +126,14 @@ class _TriangleMultiplication(nn.Module):
         if z.dim() != 4 or z.shape[1] != z.shape[2] or z.shape[3] != self.dim or z.dtype != torch.float32:
             raise ValueError(f"z must be fp32 [B, N, N, {self.dim}], got {tuple(z.shape)} {z.dtype}")
         zc = z.contiguous()
+        if dropout is not None:
+            if w_tb is not None:
+                raise _lib.TriAttnUnsupported(_lib.EUNSUPPORTED, "w_tb with dropout")
+            y = self._run(zc, mask, False, None)
+            with torch.no_grad():
+                return dropout_add_layer_norm(zc, y, ln_next.weight, ln_next.bias, dropout.p, dropout.seed, dropout.offset,
+                                           share=(2, 3) if dropout.share is None else dropout.share, eps=ln_next.eps,
+                                              out_dtype=torch.bfloat16 if dtype == _lib.BF16 else torch.float16)
         B, N = zc.shape[0], zc.shape[1]
         m = None
         if mask is not None:

@@ -299,6 +299,57 @@ TRIATTN_API int triattn_forward_noalloc(const float* z, const float* mask, const
                                         int starting, float inf, int dtype, int add_residual, float* out,
                                         void* stream);
 
+/* ---- residual path of the pair stack: LayerNorm, dropout, residual add, and their gradients ---
+ * What stands between two pair layers, as calls of their own: the LayerNorm that feeds a layer
+ * (boltz_mlx/layers/norm.py:8-17, kernels.py:438-507; with a 16-bit out its `.f16()`, :254-263), the
+ * dropout that training puts on a layer's update (the reference is inference only and has none), and
+ * the two with the residual add in one pass (the hand-over of kernels.py:1448-1480, with dropout).
+ *
+ * Tensors are [shape[0]][shape[1]][shape[2]][dim] with unit stride along dim.  shape and the strides
+ * (elements, leading three axes; NULL = dense) are HOST arrays; a stride may be 0 in a tensor that is
+ * only read.  x / z are the residual stream.  Types: stream fp32 with an fp32 or 16-bit result, or one
+ * 16-bit type throughout; y in the stream's type or the result's; weight, bias and their gradients in
+ * param_dtype.  weight NULL = ones, bias NULL = zeros.  dim up to 8192 (triattn_dropout_add: 2^30), fewer
+ * than 2^31 - 2^20 rows; an empty axis makes the call empty.  Statistics and sums are fp32.
+ *
+ * Dropout: element e of the mask tensor (the tensor's shape with size 1 along every axis k whose bit k
+ * is set in `share`; bit 3 = the channels) takes word e % 4 of Philox4x32-10 with key = seed and
+ * counter = (e / 4, offset), and is dropped if that word is below round(p * 2^32).  Kept values are
+ * scaled by fp32(1 / (1 - p)); a dropped value contributes nothing, even where y is not finite; p = 1
+ * drops everything.  The mask is never stored: the same seed and offset give it again.  rng_state:
+ * NULL, or a DEVICE array {seed, offset} that is read instead when the kernel runs (a captured graph
+ * then draws anew on each replay). */
+TRIATTN_API int triattn_layer_norm(const void* x, int x_dtype, const int64_t* x_strides, const int64_t* shape,
+                                   int64_t dim, const void* weight, const void* bias, int param_dtype, float eps,
+                                   void* out, int out_dtype, const int64_t* out_strides, float* mean, float* rstd,
+                                   void* stream); /* mean, rstd: [rows] for the backward pass, or NULL */
+/* out = z + dropout(y) (out in z's type, may alias z with the same strides), or dropout(y) with z NULL */
+TRIATTN_API int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, const void* y, int y_dtype,
+                                    const int64_t* y_strides, const int64_t* shape, int64_t dim, int share, double p,
+                                    uint64_t seed, uint64_t offset, const uint64_t* rng_state, void* out, int out_dtype,
+                                    const int64_t* out_strides, void* stream);
+/* sum = z + dropout(y) in z's type (may alias z with the same strides), out = LayerNorm(sum) */
+TRIATTN_API int triattn_dropout_add_layer_norm(const void* z, int z_dtype, const int64_t* z_strides, const void* y,
+                                               int y_dtype, const int64_t* y_strides, const int64_t* shape, int64_t dim,
+                                               int share, double p, uint64_t seed, uint64_t offset,
+                                               const uint64_t* rng_state, const void* weight, const void* bias,
+                                               int param_dtype, float eps, void* sum, const int64_t* sum_strides,
+                                               void* out, int out_dtype, const int64_t* out_strides, float* mean,
+                                               float* rstd, void* stream);
+/* Gradients of the two LayerNorm calls, from x (= sum), mean and rstd as the forward call left them:
+ * dx = dsum + LayerNorm'(dout) (dsum: gradient of sum from elsewhere, or NULL), dy = dropout'(dx),
+ * dweight, dbias.  Each of dx, dy (dense), dweight and dbias may be NULL.  The workspace (16-byte
+ * aligned, for dweight / dbias only) holds one partial row of column sums per CTA; they are summed in a
+ * fixed order, so that the same call gives the same bits. */
+TRIATTN_API size_t triattn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
+TRIATTN_API int triattn_layer_norm_backward(const void* dout, int dout_dtype, const int64_t* dout_strides,
+                                            const void* x, int x_dtype, const int64_t* x_strides, const int64_t* shape,
+                                            int64_t dim, const void* weight, int param_dtype, const float* mean,
+                                            const float* rstd, const void* dsum, const int64_t* dsum_strides, int share,
+                                            double p, uint64_t seed, uint64_t offset, const uint64_t* rng_state,
+                                            void* dx, void* dy, int y_dtype, void* dweight, void* dbias, void* workspace,
+                                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
