@@ -7,11 +7,13 @@ missing, `lib()` raises ImportError; if a CUDA tensor is not supplied, the wrapp
 from __future__ import annotations
 
 import ctypes
+import importlib
 from pathlib import Path
 
 import torch
 
 LIB_PATH = Path(__file__).with_name("libtriattn.so")
+RESIDUAL_PATH = Path(__file__).with_name("_residual.so")
 
 OK, EINVAL, EUNSUPPORTED, ECUDA, EDEVICE, ENOSPACE = 0, 1, 2, 3, 4, 5
 F32, F16, BF16 = 0, 1, 2
@@ -120,6 +122,20 @@ def lib() -> ctypes.CDLL:
                 getattr(L, name).restype = ctypes.c_int
         _L = L
     return _L
+
+
+_R = None
+
+
+def residual():
+    """The compiled binding of the residual path (csrc/torch_residual.cpp): tensors and gradients over lib()."""
+    global _R
+    if _R is None:
+        if not RESIDUAL_PATH.exists():
+            raise ImportError(f"{RESIDUAL_PATH} is not built; run `python -m boltz_mlx_b200.build`")
+        lib()
+        _R = importlib.import_module("boltz_mlx_b200._residual")
+    return _R
 
 
 def check(rc: int) -> None:

@@ -1,4 +1,5 @@
-"""Build libtriattn.so in-tree with nvcc for sm_100a (cross-compiles without a GPU).
+"""Build libtriattn.so in-tree with nvcc for sm_100a (cross-compiles without a GPU), and the PyTorch binding of
+the residual path, _residual.so, with g++ over it.
 
     python -m boltz_mlx_b200.build            # or: python boltz_mlx_b200/build.py
 """
@@ -8,12 +9,15 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtriattn.so"
+RESIDUAL = PKG / "_residual.so"
+RESIDUAL_SOURCE = CSRC / "torch_residual.cpp"
 SOURCES = ["capi.cu", "kernels_f32.cu", "kernels_tc.cu", "noalloc.cu", "peer.cu", "trimul.cu",
            "residual_capi.cu", "residual_fwd.cu", "residual_bwd.cu", "dropout_add.cu"]
 HEADERS = ["sm100.cuh", "triattn_internal.cuh", "residual.cuh"]
@@ -35,26 +39,44 @@ def nvcc() -> str:
     return cand if Path(cand).exists() else "nvcc"
 
 
+def _older(target: Path, deps: list[Path]) -> bool:
+    return not target.exists() or any(d.stat().st_mtime > target.stat().st_mtime for d in deps)
+
+
 def stale() -> bool:
-    if not LIB.exists():
-        return True
-    t = LIB.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES + HEADERS] + [ROOT / "include" / "triattn.h"]
-    return any(d.stat().st_mtime > t for d in deps)
+    return _older(LIB, [CSRC / s for s in SOURCES + HEADERS] + [ROOT / "include" / "triattn.h"])
 
 
-def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
-    if not force and not stale():
-        return LIB
-    cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", str(ROOT / "include"), "-I", str(CSRC),
-           "-o", str(LIB), *[str(CSRC / s) for s in SOURCES]]
+def residual_command() -> list[str]:
+    import torch
+
+    at = Path(torch.__file__).parent
+    cuda = Path(nvcc()).resolve().parents[1] if Path(nvcc()).exists() else Path("/usr/local/cuda")
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_residual",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-I{at / 'include'}",
+            f"-I{at / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{cuda / 'include'}",
+            f"-I{sysconfig.get_paths()['include']}", f"-I{ROOT / 'include'}", str(RESIDUAL_SOURCE), "-o", str(RESIDUAL),
+            f"-L{at / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10",
+            "-lc10_cuda", f"-L{PKG}", "-ltriattn", "-Wl,-rpath,$ORIGIN"]
+
+
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
     if verbose and (r.stdout or r.stderr):
         print(r.stdout, r.stderr)
+
+
+def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
+    if force or stale():
+        _run([nvcc(), *NVCC_FLAGS, *(extra or []), "-I", str(ROOT / "include"), "-I", str(CSRC),
+              "-o", str(LIB), *[str(CSRC / s) for s in SOURCES]], verbose)
+    if force or _older(RESIDUAL, [RESIDUAL_SOURCE, ROOT / "include" / "triattn.h"]):
+        _run(residual_command(), verbose)
     return LIB
 
 

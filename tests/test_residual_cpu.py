@@ -94,10 +94,8 @@ def test_division_by_invariant():
             assert fast(n, d) == n // d, (n, d)
 
 
-# ---- shapes, strides, shared axes -----------------------------------------------------------------------
-def test_shape_and_share_of_fewer_and_more_axes():
-    arr, rows, dim = residual._shape3((5, 7, 3))
-    assert list(arr) == [1, 5, 7] and (rows, dim) == (35, 3)
+# ---- shared axes ----------------------------------------------------------------------------------------
+def test_share_of_fewer_and_more_axes():
     assert residual._share((2, 3), 4) == 0b1100 and residual._share([-1], 2) == 0b1000 and residual._share((), 4) == 0
     assert residual._share((0,), 2) == 0b0100
     assert residual._share((0, 1), 5) == 0b0001 and residual._share((2, 4), 5) == 0b1010
@@ -105,59 +103,78 @@ def test_shape_and_share_of_fewer_and_more_axes():
         residual._share((0,), 5)
     with pytest.raises(ValueError):
         residual._share((4,), 4)
-    t = torch.zeros(2, 3, 4, 8).transpose(1, 2)
-    u, st = residual._rows(t)
-    assert u is t and list(st) == [96, 8, 32]
-    u, st = residual._rows(torch.zeros(4, 8).t())
-    assert u.is_contiguous() and st is None
 
 
-# ---- refusals -------------------------------------------------------------------------------------------
-def test_calls_refuse_cpu_tensors():
+# ---- refusals: what can be refused anywhere comes before "needs CUDA tensors" ---------------------------
+def _calls(z, y, p=0.1, seed=1, offset=0, **kw):
+    """dropout_add and dropout_add_layer_norm on the same arguments"""
+    yield lambda: b200.dropout_add(z, y, p, seed, offset, **kw)
+    yield lambda: b200.dropout_add_layer_norm(z, y, None, None, p, seed, offset, **kw)
+
+
+def test_calls_refuse_cpu_tensors(L):
     x = torch.zeros(2, 8)
-    for f in (lambda: b200.layer_norm(x), lambda: b200.dropout(x, 0.1, 1), lambda: b200.dropout_add(x, x, 0.1, 1),
-              lambda: b200.dropout_add_layer_norm(x, x, None, None, 0.1, 1), lambda: b200.LayerNorm(8)(x)):
+    for f in (lambda: b200.layer_norm(x), lambda: b200.dropout(x, 0.1, 1), *_calls(x, x), lambda: b200.LayerNorm(8)(x),
+              lambda: b200.dropout_add(x, x, 0.1, 1, inplace=True), lambda: b200.layer_norm(x, torch.ones(8), torch.ones(8))):
         with pytest.raises(RuntimeError, match="CUDA"):
             f()
 
 
-def test_argument_checks():
-    dev = torch.device("cpu")
-    for p in (-0.1, 1.5, float("nan")):
+def test_numbers_are_refused(L):
+    x = torch.zeros(2, 8)
+    for kw in ({"p": -0.1}, {"p": 1.5}, {"p": float("nan")}, {"seed": -1}, {"seed": 1 << 64}, {"offset": -1},
+               {"offset": 1 << 64}, {"share": (2,)}, {"share": (-3,)}, {"seed": torch.zeros(3, dtype=torch.int64)},
+               {"seed": torch.zeros(2)}, {"seed": torch.zeros(4, dtype=torch.int64)[::2]},
+               {"seed": torch.zeros(2, dtype=torch.int64), "offset": 5}):
+        for f in _calls(x, x, **kw):
+            with pytest.raises(ValueError):
+                f()
+        if "share" not in kw:
+            kw = {"p": 0.1, "seed": 1, **kw}
+            with pytest.raises(ValueError):
+                b200.dropout(x, **kw)
+    assert residual._draw("f", 0.4, 1, 2, False)[0] == 0.0
+
+
+def test_tensors_are_refused(L):
+    z = torch.zeros(2, 8)
+    for a, b in ((z, z[:1]), (z, torch.zeros(8)), (torch.zeros(()), torch.zeros(())), (z[:, :0], z[:, :0])):
+        for f in _calls(a, b):
+            with pytest.raises(ValueError):
+                f()
+    for a, b in ((z.half(), z), (z.half(), z.bfloat16()), (z.double(), z.double()), (z, z.long())):
+        for f in _calls(a, b):
+            with pytest.raises(NotImplementedError):
+                f()
+    bad = [(z, torch.zeros(7), None), (z, None, torch.zeros(7)), (z, torch.zeros(1, 8), None),
+           (z, torch.zeros(8), torch.zeros(8).half()), (torch.zeros(()), None, None), (z[:, :0], None, None)]
+    for x, w, b in bad:
         with pytest.raises(ValueError):
-            residual._draw("f", p, 1, 0, dev, True)
-    for seed, offset in ((-1, 0), (1 << 64, 0), (0, -1), (0, 1 << 64)):
-        with pytest.raises(ValueError):
-            residual._draw("f", 0.1, seed, offset, dev, True)
+            b200.layer_norm(x, w, b)
     with pytest.raises(ValueError):
-        residual._draw("f", 0.1, torch.zeros(3, dtype=torch.int64), 0, dev, True)
+        b200.dropout_add_layer_norm(z, z, torch.zeros(7), None, 0.1, 1)
     with pytest.raises(ValueError):
-        residual._draw("f", 0.1, torch.zeros(2), 0, dev, True)
+        b200.dropout_add_layer_norm(z, z, None, None, 0.1, 1, trans_out=True)
+    for f in (lambda: b200.layer_norm(z, torch.zeros(8).double()), lambda: b200.layer_norm(torch.zeros(1, 8193)),
+              lambda: b200.dropout_add_layer_norm(torch.zeros(1, 8193), torch.zeros(1, 8193), None, None, 0.1, 1),
+              lambda: b200.layer_norm(z.long()), lambda: b200.layer_norm(z, out_dtype=torch.float64),
+              lambda: b200.dropout_add_layer_norm(z.half(), z.half(), None, None, 0.1, 1, out_dtype=torch.bfloat16),
+              lambda: b200.LayerNorm((4, 8)),
+              lambda: b200.TriangleAttention(precision="fp32").norm_input(torch.zeros(1, 4, 4, 128))):
+        with pytest.raises(NotImplementedError):
+            f()
     with pytest.raises(ValueError):
-        residual._draw("f", 0.1, torch.zeros(2, dtype=torch.int64), 5, dev, True)
-    assert residual._draw("f", 0.4, 1, 2, dev, False)[0] == 0.0
-    with pytest.raises(ValueError):
-        residual._params("f", torch.zeros(7), None, 8)
-    with pytest.raises(ValueError):
-        residual._params("f", torch.zeros(8), torch.zeros(8, dtype=torch.float16), 8)
-    with pytest.raises(NotImplementedError):
-        residual._params("f", torch.zeros(8, dtype=torch.float64), None, 8)
-    with pytest.raises(NotImplementedError):
-        residual._check_dim("f", torch.zeros(1, 8193))
-    with pytest.raises(ValueError):
-        residual._check_dim("f", torch.zeros(3, 0))
-    with pytest.raises(ValueError):
-        residual._check_pair("f", torch.zeros(2, 8), torch.zeros(1, 8))
-    with pytest.raises(NotImplementedError):
-        residual._check_pair("f", torch.zeros(2, 8, dtype=torch.float16), torch.zeros(2, 8))
-    with pytest.raises(NotImplementedError):
-        residual._code(torch.zeros(2, dtype=torch.int32), "x")
-    with pytest.raises(NotImplementedError):
-        b200.LayerNorm((4, 8))
-    with pytest.raises(ValueError):
-        b200.LayerNorm(8)._check(torch.zeros(2, 9))
-    with pytest.raises(NotImplementedError):
-        b200.TriangleAttention(precision="fp32").norm_input(torch.zeros(1, 4, 4, 128))
+        b200.LayerNorm(8)(torch.zeros(2, 9))
+
+
+def test_in_place_is_refused(L):
+    sq = torch.zeros(3, 3, 8)
+    with pytest.raises(ValueError, match="overlaps"):
+        b200.dropout_add(sq, sq.transpose(0, 1), 0.1, 1, inplace=True)
+    with pytest.raises(ValueError, match="dense last axis"):
+        b200.dropout_add(torch.zeros(8, 4).t(), torch.zeros(4, 8), 0.1, 1, inplace=True)
+    with pytest.raises(RuntimeError, match="gradients"):
+        b200.dropout_add(sq.clone().requires_grad_(), sq, 0.1, 1, inplace=True)
 
 
 A = 4096  # an address that validation may look at but nothing may touch
