@@ -19,10 +19,13 @@ __device__ __forceinline__ uint64_t mask_pos(const DropoutAddArgs& a, uint32_t r
 
 template <class T, int VEC>
 __device__ __forceinline__ void load_some(Pack<T, VEC>& r, const T* p, int n) {
-  if (VEC == 1 || n == VEC)
+  if (VEC == 1 || n == VEC) {
     r = load_pack<T, VEC>(p);
-  else
-    for (int k = 0; k < n; ++k) r.v[k] = p[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (k < n) r.v[k] = p[k];
+  }
 }
 
 template <class TZ, class TY, class TO, int VEC, bool FLAT, bool HASZ>
@@ -69,10 +72,9 @@ __global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddA
         const uint32_t t = rest + q, dr = per_row.div(t);
         row = row_base + dr;
         col = (t - dr * per_row.d) * VEC;
-        const RowIndex i = a.map.at(row);
-        zo = row_offset(a.zs, row, i, D) + col;
-        yo = row_offset(a.ys, row, i, D) + col;
-        oo[u] = row_offset(a.os, row, i, D) + col;
+        zo = row_offset(a.zs, row, a.map, D) + col;
+        yo = row_offset(a.ys, row, a.map, D) + col;
+        oo[u] = row_offset(a.os, row, a.map, D) + col;
       }
       if (HASZ && !a.in_place) load_some(zr[u], z + zo, n[u]);
       if (a.drop.on) {
@@ -129,10 +131,13 @@ __global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddA
         }
         o.v[k] = from_f32<TO>(f);
       }
-      if (VEC == 1 || n[u] == VEC)
+      if (VEC == 1 || n[u] == VEC) {
         store_pack(out + oo[u], o);
-      else
-        for (int k = 0; k < n[u]; ++k) out[oo[u] + k] = o.v[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (k < n[u]) out[oo[u] + k] = o.v[k];
+      }
     }
   }
 }

@@ -16,15 +16,21 @@ namespace {
 
 constexpr int kCtasPerSm = 4;
 
-template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, bool HASY>
-__global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwdArgs a) {
+template <class TX, class TO, int VEC, int NCH, int R, bool HASY>
+constexpr int stage_bytes(int width, int dim) {
+  return R * ((HASY ? 2 : 1) * row_slot<TX, VEC, NCH>(width, dim) + row_slot<TO, VEC, NCH>(width, dim));
+}
+
+template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY>
+__global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwdArgs a, int width) {
   constexpr int EPL = VEC * NCH;
-  extern __shared__ float colsum[];  // LPR: [warps][2][dim] of the column sums
-  __shared__ float red[LPR ? 1 : 2 * 2 * RES_MAX_WARPS];
+  extern __shared__ __align__(16) char smem[];  // the groups' stages; at the end [groups][2][dim] column sums
+  using L = Lanes<VEC, LPR, NCH>;
+  __shared__ float red[L::red_floats];
   int phase = 0;
-  const int width = LPR ? LPR : blockDim.x;
-  const int lane = LPR ? threadIdx.x & (width - 1) : threadIdx.x;
-  const int group = LPR ? threadIdx.x / width : 0, groups = LPR ? blockDim.x / width : 1;
+  const L l(a.dim, width);
+  using CX = RowCopy<TX, VEC, LPR, NCH>;
+  using CO = RowCopy<TO, VEC, LPR, NCH>;
   const int D = a.dim;
   const float inv_d = 1.0f / (float)D;
   const TX* x = static_cast<const TX*>(a.x);
@@ -33,164 +39,195 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
   TX* dx = static_cast<TX*>(a.dx);
   TY* dy = static_cast<TY*>(a.dy);
 
-  bool act[NCH];
   float w[EPL], dw[EPL], db[EPL];
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int col = (lane + c * width) * VEC;
-    act[c] = col < D;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      w[c * VEC + v] = act[c] ? load_param(a.weight, a.param_dtype, col + v, 1.0f) : 0.0f;
-      dw[c * VEC + v] = db[c * VEC + v] = 0.0f;
-    }
+  for (int i = 0; i < EPL; ++i) {
+    w[i] = l.act[i / VEC] ? load_param(a.weight, a.param_dtype, l.col(i / VEC) + i % VEC, 1.0f) : 0.0f;
+    dw[i] = db[i] = 0.0f;
   }
   const Philox rng(a.drop);
+  const bool has_ds = HASY && ds, has_dy = HASY && dy;
+  const bool row_draw = has_dy && a.drop.on && !a.drop.per_channel, draw = has_dy && a.drop.on && a.drop.per_channel;
 
-  const uint32_t step = gridDim.x * groups * R;
-  for (uint32_t base = blockIdx.x * groups * R; base < a.map.rows; base += step) {
-    const uint32_t row0 = base + group * R;
-    RowIndex idx[R];
-    Pack<TX, VEC> xr[R][NCH], sr[R][NCH];
-    Pack<TO, VEC> gr[R][NCH];
-    float mean[R], rstd[R];
+  const int slot_x = row_slot<TX, VEC, NCH>(l.width, D), slot_o = row_slot<TO, VEC, NCH>(l.width, D);
+  const int stage = stage_bytes<TX, TO, VEC, NCH, R, HASY>(l.width, D);
+  char* ring = smem + l.group * S * stage;
+  const uint32_t ring32 = smem_u32(ring);
+
+  const uint32_t rows = a.map.rows, step = gridDim.x * l.groups * R;
+  const auto issue = [&](uint32_t base, int s) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t row = row0 + r;
-      const bool live = row < a.map.rows;
-      idx[r] = a.map.at(live ? row : a.map.rows - 1);
-      const TX* px = x + row_offset(a.xs, row, idx[r], D);
-      const TO* pg = dout + row_offset(a.dos, row, idx[r], D);
-      const TX* ps = ds + (HASY && ds ? row_offset(a.dss, row, idx[r], D) : 0);
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const int col = (lane + c * width) * VEC;
-        if (act[c] && live) {
-          xr[r][c] = load_pack<TX, VEC>(px + col);
-          gr[r][c] = load_pack<TO, VEC>(pg + col);
-          if (HASY && ds) sr[r][c] = load_pack<TX, VEC>(ps + col);
-        }
-      }
-      mean[r] = live ? a.mean[row] : 0.0f;
-      rstd[r] = live ? a.rstd[row] : 0.0f;
+      const uint32_t row = base + l.group * R + r;
+      if (row >= rows) continue;
+      const uint32_t at = ring32 + s * stage;
+      CX::issue(l, at + r * slot_x, x + row_offset(a.xs, row, a.map, D));
+      CO::issue(l, at + R * slot_x + r * slot_o, dout + row_offset(a.dos, row, a.map, D));
+      if constexpr (HASY)
+        if (has_ds) CX::issue(l, at + R * (slot_x + slot_o) + r * slot_x, ds + row_offset(a.dss, row, a.map, D));
     }
+  };
+  float mean[R], rstd[R], mean_next[R], rstd_next[R];  // of the batch in hand and of the next one
+  const auto statistics = [&](uint32_t base) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint32_t row = base + l.group * R + r;
+      mean_next[r] = row < rows ? a.mean[row] : 0.0f;
+      rstd_next[r] = row < rows ? a.rstd[row] : 0.0f;
+    }
+  };
+
+  uint32_t ahead = blockIdx.x * l.groups * R;
+  statistics(ahead);
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s, ahead += step) {
+    if (ahead < rows) issue(ahead, s);
+    copy_commit();
+  }
+  int s = 0;
+  for (uint32_t base = blockIdx.x * l.groups * R; base < rows; base += step, ahead += step) {
+    if (ahead < rows) issue(ahead, s == 0 ? S - 1 : s - 1);
+    copy_commit();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = mean_next[r];
+      rstd[r] = rstd_next[r];
+    }
+    statistics(base + step);
+    copy_wait<S - 1>();
+    l.sync();
+    const uint32_t row0 = base + l.group * R;
+    const char* here = ring + s * stage;
     // v[2 r] = sum g, v[2 r + 1] = sum g xh
     float xh[R][EPL], g[R][EPL], v[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool live = row0 + r < a.map.rows;
+      const uint32_t row = row0 + r;
+      const bool live = row < rows;
+      const TX* xrow = x + (VEC == 1 ? row_offset(a.xs, row, a.map, D) : 0);
+      const TO* orow = dout + (VEC == 1 ? row_offset(a.dos, row, a.map, D) : 0);
       v[2 * r] = v[2 * r + 1] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        const bool in = act[i / VEC] && live;
-        const float d = in ? to_f32(gr[r][i / VEC].v[i % VEC]) : 0.0f;
-        xh[r][i] = in ? (to_f32(xr[r][i / VEC].v[i % VEC]) - mean[r]) * rstd[r] : 0.0f;
-        dw[i] = fmaf(d, xh[r][i], dw[i]);
-        db[i] += d;
-        g[r][i] = d * w[i];
-        v[2 * r] += g[r][i];
-        v[2 * r + 1] = fmaf(g[r][i], xh[r][i], v[2 * r + 1]);
+      for (int c = 0; c < NCH; ++c) {
+        float xv[VEC], dv[VEC];
+        const bool in = live && l.act[c];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) xv[k] = mean[r], dv[k] = 0.0f;
+        if (in) {
+          CX::read(l, here + r * slot_x, xrow, c, xv);
+          CO::read(l, here + R * slot_x + r * slot_o, orow, c, dv);
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const int i = c * VEC + k;
+          xh[r][i] = (xv[k] - mean[r]) * rstd[r];
+          dw[i] = fmaf(dv[k], xh[r][i], dw[i]);
+          db[i] += dv[k];
+          g[r][i] = dv[k] * w[i];
+          v[2 * r] += g[r][i];
+          v[2 * r + 1] = fmaf(g[r][i], xh[r][i], v[2 * r + 1]);
+        }
       }
     }
-    row_sum<LPR, 2 * R>(v, red, phase);
-    bool keep_row[R];
+    l.sum(v, red, phase);
+    uint32_t whole = ~0u;  // bit r: row r is not dropped whole
     if constexpr (HASY) {
-      if (dy && a.drop.on && !a.drop.per_channel) {
+      if (row_draw) {
         if constexpr (LPR && R > 1) {
-          const int mine = lane & (R - 1);
-          uint64_t pos = 0;
+          const uint32_t row = row0 + (l.lane & (R - 1));
+          const bool k = row < rows && rng.word(mask_base(a.drop, a.map.at(row))) > a.drop.drop_max;
+          whole = 0;
+#pragma unroll
+          for (int r = 0; r < R; ++r) whole |= __shfl_sync(0xffffffffu, (uint32_t)k, r, LPR) << r;
+        } else {
+          whole = 0;
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            if (r == mine) pos = mask_base(a.drop, idx[r]);
-          const bool k = rng.word(pos) > a.drop.drop_max;
-#pragma unroll
-          for (int r = 0; r < R; ++r) keep_row[r] = __shfl_sync(0xffffffffu, (int)k, r, LPR) != 0;
-        } else {
-#pragma unroll
-          for (int r = 0; r < R; ++r) keep_row[r] = rng.word(mask_base(a.drop, idx[r])) > a.drop.drop_max;
+            if (row0 + r < rows && rng.word(mask_base(a.drop, a.map.at(row0 + r))) > a.drop.drop_max) whole |= 1u << r;
         }
-      } else {
-#pragma unroll
-        for (int r = 0; r < R; ++r) keep_row[r] = true;
       }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint32_t row = row0 + r;
-      if (row >= a.map.rows) continue;
+      const bool live = row < rows;
       const float c1 = v[2 * r] * inv_d, c2 = v[2 * r + 1] * inv_d;
-      const uint64_t mb = mask_base(a.drop, idx[r]);
+      uint32_t keep[NCH];
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) keep[c] = whole >> r & 1 ? 0xffu : 0u;
+      if constexpr (HASY)
+        if (draw) keep_pieces(l, rng, mask_base(a.drop, a.map.at(live ? row : rows - 1)), a.drop.drop_max, keep);
+      const TX* srow = ds + (HASY && VEC == 1 && has_ds ? row_offset(a.dss, row, a.map, D) : 0);
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        if (!act[c]) continue;
-        const int col = (lane + c * width) * VEC;
-        Pack<TX, VEC> o;
-        float f[VEC];
+        if (!live || !l.act[c]) continue;
+        const int col = l.col(c);
+        float f[VEC], sv[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           const int i = c * VEC + k;
           f[k] = rstd[r] * (g[r][i] - c1 - xh[r][i] * c2);
-          if (HASY && ds) f[k] += to_f32(sr[r][c].v[k]);
-          o.v[k] = from_f32<TX>(f[k]);
         }
-        if (dx) store_pack(dx + (int64_t)row * D + col, o);
+        if constexpr (HASY) {
+          if (has_ds) {
+            CX::read(l, here + R * (slot_x + slot_o) + r * slot_x, srow, c, sv);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) f[k] += sv[k];
+          }
+        }
+        if (dx) {
+          Pack<TX, VEC> o;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) o.v[k] = from_f32<TX>(f[k]);
+          store_pack(dx + (int64_t)row * D + col, o);
+        }
         if constexpr (HASY) {
           if (dy) {
-            uint32_t bits = keep_row[r] ? 0xffu : 0u;
-            if (a.drop.on && a.drop.per_channel) bits = keep_bits<VEC>(rng, mb + col, a.drop.drop_max);
             Pack<TY, VEC> q;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) q.v[k] = from_f32<TY>(bits >> k & 1 ? f[k] * a.drop.scale : 0.0f);
+            for (int k = 0; k < VEC; ++k) q.v[k] = from_f32<TY>(keep[c] >> k & 1 ? f[k] * a.drop.scale : 0.0f);
             store_pack(dy + (int64_t)row * D + col, q);
           }
         }
       }
     }
+    l.sync();
+    s = s == S - 1 ? 0 : s + 1;
   }
+  copy_wait<0>();
 
   if (!a.partial) return;
+  // groups of one warp first (they own the same channels), then all groups through shared memory
   float* part = a.partial + (size_t)blockIdx.x * 2 * D;
-  if constexpr (LPR == 0) {
+#pragma unroll
+  for (int o = LPR ? LPR : 32; o < 32; o <<= 1) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
+      db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+    }
+  }
+  const int sets = LPR ? blockDim.x >> 5 : l.groups;
+  const bool writes = LPR ? (threadIdx.x & 31) < LPR : true;
+  float* mine = sets == 1 ? part : reinterpret_cast<float*>(smem) + (size_t)(LPR ? threadIdx.x >> 5 : l.group) * 2 * D;
+  __syncthreads();  // every warp has read its last rows
+  if (writes) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
-      if (act[c]) {
+      if (l.act[c]) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const int col = (lane + c * width) * VEC + v;
-          part[col] = dw[c * VEC + v];
-          part[D + col] = db[c * VEC + v];
+        for (int k = 0; k < VEC; ++k) {
+          mine[l.col(c) + k] = dw[c * VEC + k];
+          mine[D + l.col(c) + k] = db[c * VEC + k];
         }
       }
-  } else {
-    // groups of one warp first (they own the same channels), then the warps through shared memory
-#pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) {
-        dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-        db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
-      }
-    }
-    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    float* mine = colsum + (size_t)warp * 2 * D;
-    if ((threadIdx.x & 31) < LPR) {
-#pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        if (act[c]) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            const int col = (lane + c * width) * VEC + v;
-            mine[col] = dw[c * VEC + v];
-            mine[D + col] = db[c * VEC + v];
-          }
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
-      float s = 0.0f;
-      for (int k = 0; k < warps; ++k) s += colsum[(size_t)k * 2 * D + i];
-      part[i] = s;
-    }
+  }
+  if (sets == 1) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+    float t = 0.0f;
+    for (int k = 0; k < sets; ++k) t += reinterpret_cast<const float*>(smem)[(size_t)k * 2 * D + i];
+    part[i] = t;
   }
 }
 
@@ -218,17 +255,17 @@ __global__ void __launch_bounds__(512) norm_bwd_join_kernel(const float* __restr
   }
 }
 
-template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, bool HASY>
-cudaError_t launch_one(const NormBwdArgs& a, int threads, cudaStream_t st) {
-  auto kernel = norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, HASY>;
-  const int per_cta = (LPR ? threads / (LPR ? LPR : 1) : 1) * R;
-  const long long need = ((long long)a.map.rows + per_cta - 1) / per_cta;
-  const long long cap = (long long)device_sm_count() * (threads > 256 ? 2 : kCtasPerSm);
-  const unsigned grid = (unsigned)(need < cap ? need : cap);
-  const size_t smem = LPR && a.partial ? (size_t)(threads / 32) * 2 * a.dim * 4 : 0;  // at most 32 KB: dim <= 512
-  kernel<<<grid, threads, smem, st>>>(a);
-  if (!a.partial) return cudaGetLastError();
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY>
+cudaError_t launch_one(const NormBwdArgs& a, int width, int threads, cudaStream_t st) {
+  static KernelInfo info;
+  const int groups = threads / width, sets = LPR ? threads / 32 : groups;
+  size_t smem = (size_t)groups * S * stage_bytes<TX, TO, VEC, NCH, R, HASY>(width, a.dim);
+  if (const size_t sums = (size_t)sets * 2 * a.dim * 4; sets > 1 && smem < sums) smem = sums;
+  unsigned grid = 0;
+  if (cudaError_t e = launch_rows(info, norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY>, a, width, groups * R, threads,
+                                  smem, kCtasPerSm, st, &grid);
+      e != cudaSuccess || !a.partial)
+    return e;
   const int blocks = (2 * a.dim + 31) / 32;
   if (a.param_dtype == DT_F32)
     norm_bwd_join_kernel<<<blocks, 512, 0, st>>>(a.partial, (int)grid, a.dim, static_cast<float*>(a.dweight),
@@ -244,27 +281,34 @@ cudaError_t launch_one(const NormBwdArgs& a, int threads, cudaStream_t st) {
 
 template <class TX, class TY, class TO, int VEC, bool HASY>
 cudaError_t launch_vec(const NormBwdArgs& a, cudaStream_t st) {
-  constexpr int M = 16 / VEC;
   const int C = (a.dim + VEC - 1) / VEC;
   if constexpr (VEC > 1) {
-    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, 2, HASY>(a, 256, st);
-    if (C <= 16) return launch_one<TX, TY, TO, VEC, 16, 1, 2, HASY>(a, 256, st);
-    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, 2, HASY>(a, 256, st);
-    if (C <= 64) return launch_one<TX, TY, TO, VEC, 32, 2, 1, HASY>(a, 256, st);
-    if constexpr (VEC == 4)
-      if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, HASY>(a, 256, st);
+    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, 2, 3, HASY>(a, 8, 256, st);
+    if (C <= 16) return launch_one<TX, TY, TO, VEC, 16, 1, 2, 3, HASY>(a, 16, 256, st);
+    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, 2, 3, HASY>(a, 32, 256, st);
+    if (C <= 64) return launch_one<TX, TY, TO, VEC, 32, 2, 1, 3, HASY>(a, 32, 256, st);
+    if constexpr (VEC == 4) {
+      if (C <= 96) return launch_one<TX, TY, TO, VEC, 32, 3, 1, 3, HASY>(a, 32, 256, st);
+      if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, 3, HASY>(a, 32, 256, st);
+    }
   } else {
-    if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 2, HASY>(a, 256, st);
-    if (C <= 512) return launch_one<TX, TY, TO, VEC, 32, 16, 1, HASY>(a, 256, st);
+    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, 2, 3, HASY>(a, 8, 256, st);
+    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, 2, 3, HASY>(a, 32, 256, st);
+    if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, 3, HASY>(a, 32, 256, st);
+    if (C <= 512) return launch_one<TX, TY, TO, VEC, 32, 16, 1, 3, HASY>(a, 32, 256, st);
   }
-  const int threads = ((C + M - 1) / M + 31) / 32 * 32;
-  return launch_one<TX, TY, TO, VEC, 0, M, 1, HASY>(a, threads, st);
+  const RowWidth w = row_width<VEC>(C);
+  if constexpr (VEC == 4)
+    if (w.pieces == 3) return launch_one<TX, TY, TO, VEC, 0, 3, 1, 2, HASY>(a, w.width, w.threads, st);
+  return launch_one<TX, TY, TO, VEC, 0, 16 / VEC, 1, 2, HASY>(a, w.width, w.threads, st);
 }
 
 template <class TX, class TY, class TO, bool HASY>
 cudaError_t launch_types(const NormBwdArgs& a, int vec, cudaStream_t st) {
-  constexpr int FULL = sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2 ? 8 : 4;
-  if (vec >= FULL) return launch_vec<TX, TY, TO, FULL, HASY>(a, st);
+  if constexpr (sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2) {
+    if (vec == 8) return launch_vec<TX, TY, TO, 8, HASY>(a, st);
+  }
+  if (vec >= 4) return launch_vec<TX, TY, TO, 4, HASY>(a, st);
   return launch_vec<TX, TY, TO, 1, HASY>(a, st);
 }
 

@@ -1,23 +1,28 @@
 // LayerNorm forward, alone or behind dropout + residual add (residual.cuh has the formulas).
 //
-// Bound by HBM: one read of every input and one write of every output; about 40 issued instructions per
-// 128-channel row against 1 KB of traffic.  A row stays in the registers of LPR lanes (or of a whole CTA
-// when it is longer than 512 channels), NCH accesses of VEC elements each, so that both statistics passes
-// (mean, then centred squares) run without a second read; R rows per group are in flight to cover the
-// latency of the loads.
+// Bound by HBM: one read of every input and one write of every output.  A persistent grid of row groups; a
+// group's next batches of R rows are on their way into shared memory (residual.cuh) while it works on one.
+// A row's values stay in registers through both statistics passes (mean, then centred squares).
 #include "residual.cuh"
 
 namespace triattn {
 namespace {
 
-template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, bool HASY>
-__global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwdArgs a) {
+template <class TX, class TY, int VEC, int NCH, int R, bool HASY>
+constexpr int stage_bytes(int width, int dim) {
+  return R * (row_slot<TX, VEC, NCH>(width, dim) + (HASY ? row_slot<TY, VEC, NCH>(width, dim) : 0));
+}
+
+template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY>
+__global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwdArgs a, int width) {
   constexpr int EPL = VEC * NCH;
-  __shared__ float red[LPR ? 1 : 2 * 2 * RES_MAX_WARPS];
+  extern __shared__ __align__(16) char smem[];  // LPR: weight and bias in fp32, then the groups' stages
+  using L = Lanes<VEC, LPR, NCH>;
+  __shared__ float red[L::red_floats];
   int phase = 0;
-  const int width = LPR ? LPR : blockDim.x;  // lanes of a row
-  const int lane = LPR ? threadIdx.x & (width - 1) : threadIdx.x;
-  const int group = LPR ? threadIdx.x / width : 0, groups = LPR ? blockDim.x / width : 1;
+  const L l(a.dim, width);
+  using CX = RowCopy<TX, VEC, LPR, NCH>;
+  using CY = RowCopy<TY, VEC, LPR, NCH>;
   const int D = a.dim;
   const float inv_d = 1.0f / (float)D;
   const TX* z = static_cast<const TX*>(a.z);
@@ -25,101 +30,128 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
   TX* sum = static_cast<TX*>(a.sum);
   TO* out = static_cast<TO*>(a.out);
 
-  bool act[NCH];
-  float w[EPL], b[EPL];
+  // Whole-CTA rows keep weight and bias in registers, rows of one warp (several at once) in shared memory.
+  float* wb = reinterpret_cast<float*>(smem);
+  const int wb_pad = LPR ? (D + VEC - 1) / VEC * VEC : 0;
+  float w[LPR ? 1 : EPL], b[LPR ? 1 : EPL];
+  if constexpr (LPR) {
+    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+      wb[i] = load_param(a.weight, a.param_dtype, i, 1.0f);
+      wb[wb_pad + i] = load_param(a.bias, a.param_dtype, i, 0.0f);
+    }
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int col = (lane + c * width) * VEC;
-    act[c] = col < D;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      w[c * VEC + v] = act[c] ? load_param(a.weight, a.param_dtype, col + v, 1.0f) : 0.0f;
-      b[c * VEC + v] = act[c] ? load_param(a.bias, a.param_dtype, col + v, 0.0f) : 0.0f;
+    for (int i = 0; i < EPL; ++i) {
+      w[i] = l.act[i / VEC] ? load_param(a.weight, a.param_dtype, l.col(i / VEC) + i % VEC, 1.0f) : 0.0f;
+      b[i] = l.act[i / VEC] ? load_param(a.bias, a.param_dtype, l.col(i / VEC) + i % VEC, 0.0f) : 0.0f;
     }
   }
   const Philox rng(a.drop);
+  const bool row_draw = HASY && a.drop.on && !a.drop.per_channel, draw = HASY && a.drop.on && a.drop.per_channel;
 
-  const uint32_t step = gridDim.x * groups * R;
-  // the loop's count is the same for every lane of a CTA (whole-warp shuffles, CTA barriers)
-  for (uint32_t base = blockIdx.x * groups * R; base < a.map.rows; base += step) {
-    const uint32_t row0 = base + group * R;
-    float x[R][EPL];
-    RowIndex idx[R];
-    Pack<TX, VEC> zr[R][NCH];
+  const int slot_x = row_slot<TX, VEC, NCH>(l.width, D), slot_y = row_slot<TY, VEC, NCH>(l.width, D);
+  const int stage = stage_bytes<TX, TY, VEC, NCH, R, HASY>(l.width, D);
+  char* ring = smem + (wb_pad * 8 + 15) / 16 * 16 + l.group * S * stage;
+  const uint32_t ring32 = smem_u32(ring);
+  uint32_t kept = ~0u;  // bit s * R + r: row r of stage s is not dropped whole
+
+  const uint32_t rows = a.map.rows, step = gridDim.x * l.groups * R;
+  const auto issue = [&](uint32_t base, int s) {
+    const uint32_t row0 = base + l.group * R;
+    if constexpr (HASY) {
+      if (row_draw) {
+        // one draw per row: lane k of a group takes that of row k, and hands it round
+        if constexpr (LPR && R > 1) {
+          const uint32_t row = row0 + (l.lane & (R - 1));
+          const bool k = row < rows && rng.word(mask_base(a.drop, a.map.at(row))) > a.drop.drop_max;
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const uint32_t bit = 1u << (s * R + r);
+            kept = __shfl_sync(0xffffffffu, (int)k, r, LPR) ? kept | bit : kept & ~bit;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const bool k = row0 + r < rows && rng.word(mask_base(a.drop, a.map.at(row0 + r))) > a.drop.drop_max;
+            const uint32_t bit = 1u << (s * R + r);
+            kept = k ? kept | bit : kept & ~bit;
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint32_t row = row0 + r;
-      idx[r] = a.map.at(row < a.map.rows ? row : a.map.rows - 1);
-      const TX* p = z + row_offset(a.zs, row, idx[r], D);
-#pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        if (act[c] && row < a.map.rows) zr[r][c] = load_pack<TX, VEC>(p + (lane + c * width) * VEC);
+      if (row >= rows) continue;
+      const uint32_t at = ring32 + s * stage + r * slot_x;
+      CX::issue(l, at, z + row_offset(a.zs, row, a.map, D));
+      if constexpr (HASY) {
+        if (kept >> (s * R + r) & 1)  // a row that is dropped whole is not read
+          CY::issue(l, ring32 + s * stage + R * slot_x + r * slot_y, y + row_offset(a.ys, row, a.map, D));
+      }
     }
-    if constexpr (HASY) {
-      Pack<TY, VEC> yr[R][NCH];
-      bool keep_row[R];
-      if (a.drop.on && !a.drop.per_channel) {
-        // one draw per row: lane k of a group takes the R rows' draws in turn and hands them round
-        bool k;
-        if constexpr (LPR && R > 1) {
-          const int mine = lane & (R - 1);
-          uint64_t pos = 0;
+  };
+
+  uint32_t ahead = blockIdx.x * l.groups * R;
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (r == mine) pos = mask_base(a.drop, idx[r]);
-          k = rng.word(pos) > a.drop.drop_max;
+  for (int s = 0; s < S - 1; ++s, ahead += step) {
+    if (ahead < rows) issue(ahead, s);
+    copy_commit();
+  }
+  int s = 0;
+  // the loop's count is the same for every lane of a CTA (whole-warp shuffles, CTA barriers)
+  for (uint32_t base = blockIdx.x * l.groups * R; base < rows; base += step, ahead += step) {
+    if (ahead < rows) issue(ahead, s == 0 ? S - 1 : s - 1);
+    copy_commit();
+    copy_wait<S - 1>();
+    l.sync();
+    const uint32_t row0 = base + l.group * R;
+    const char* here = ring + s * stage;
+    float x[R][EPL];
 #pragma unroll
-          for (int r = 0; r < R; ++r) keep_row[r] = __shfl_sync(0xffffffffu, (int)k, r, LPR) != 0;
-        } else {
+    for (int r = 0; r < R; ++r) {
+      const uint32_t row = row0 + r;
+      const bool live = row < rows;
+      const TX* zrow = z + (VEC == 1 ? row_offset(a.zs, row, a.map, D) : 0);
 #pragma unroll
-          for (int r = 0; r < R; ++r) keep_row[r] = rng.word(mask_base(a.drop, idx[r])) > a.drop.drop_max;
-        }
-      } else {
+      for (int c = 0; c < NCH; ++c) {
+        float v[VEC];
 #pragma unroll
-        for (int r = 0; r < R; ++r) keep_row[r] = true;
+        for (int k = 0; k < VEC; ++k) v[k] = 0.0f;
+        if (live && l.act[c]) CX::read(l, here + r * slot_x, zrow, c, v);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x[r][c * VEC + k] = v[k];
       }
+      if constexpr (HASY) {
+        const TY* yrow = y + (VEC == 1 ? row_offset(a.ys, row, a.map, D) : 0);
+        uint32_t keep[NCH];
+        const uint32_t whole = kept >> (s * R + r) & 1 ? 0xffu : 0u;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint32_t row = row0 + r;
-        const TY* p = y + row_offset(a.ys, row, idx[r], D);
-#pragma unroll
-        for (int c = 0; c < NCH; ++c)  // a row that is dropped whole is not read
-          if (act[c] && row < a.map.rows && keep_row[r]) yr[r][c] = load_pack<TY, VEC>(p + (lane + c * width) * VEC);
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const uint32_t row = row0 + r;
-        const bool live = row < a.map.rows;
-        const uint64_t mb = mask_base(a.drop, idx[r]);
-        TX* p = sum + row_offset(a.ss, row, idx[r], D);
+        for (int c = 0; c < NCH; ++c) keep[c] = whole;
+        if (draw) keep_pieces(l, rng, mask_base(a.drop, a.map.at(live ? row : rows - 1)), a.drop.drop_max, keep);
+        TX* p = sum + row_offset(a.ss, row, a.map, D);
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-          const int col = (lane + c * width) * VEC;
-          uint32_t bits = keep_row[r] ? 0xffu : 0u;
-          if (a.drop.on && a.drop.per_channel) bits = keep_bits<VEC>(rng, mb + col, a.drop.drop_max);
-          Pack<TX, VEC> s;
+          if (!live || !l.act[c]) continue;
+          float v[VEC];
+          if (keep[c]) {
+            CY::read(l, here + R * slot_x + r * slot_y, yrow, c, v);
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            float f = 0.0f;
-            if (act[c] && live) {
-              f = to_f32(zr[r][c].v[v]);
-              if (bits >> v & 1) f = fmaf(to_f32(yr[r][c].v[v]), a.drop.scale, f);
-            }
-            s.v[v] = from_f32<TX>(f);
-            x[r][c * VEC + v] = to_f32(s.v[v]);  // the norm is taken of the stream as it is held
+            for (int k = 0; k < VEC; ++k)
+              if (keep[c] >> k & 1) x[r][c * VEC + k] = fmaf(v[k], a.drop.scale, x[r][c * VEC + k]);
           }
-          if (act[c] && live) store_pack(p + col, s);
+          Pack<TX, VEC> o;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            o.v[k] = from_f32<TX>(x[r][c * VEC + k]);
+            x[r][c * VEC + k] = to_f32(o.v[k]);  // the norm is taken of the stream as it is held
+          }
+          store_pack(p + l.col(c), o);
         }
       }
-    } else {
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int c = 0; c < NCH; ++c)
-#pragma unroll
-          for (int v = 0; v < VEC; ++v)
-            x[r][c * VEC + v] = act[c] && row0 + r < a.map.rows ? to_f32(zr[r][c].v[v]) : 0.0f;
     }
+    l.sync();
 
     float mean[R], var[R];
 #pragma unroll
@@ -128,78 +160,104 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
 #pragma unroll
       for (int i = 0; i < EPL; ++i) mean[r] += x[r][i];
     }
-    row_sum<LPR, R>(mean, red, phase);
+    l.sum(mean, red, phase);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       mean[r] *= inv_d;
       var[r] = 0.0f;
 #pragma unroll
       for (int i = 0; i < EPL; ++i) {
-        x[r][i] = act[i / VEC] ? x[r][i] - mean[r] : 0.0f;
+        x[r][i] = l.act[i / VEC] ? x[r][i] - mean[r] : 0.0f;
         var[r] = fmaf(x[r][i], x[r][i], var[r]);
       }
     }
-    row_sum<LPR, R>(var, red, phase);
+    l.sum(var, red, phase);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const uint32_t row = row0 + r;
-      if (row >= a.map.rows) continue;
-      const float rstd = rsqrtf(fmaf(var[r], inv_d, a.eps));
-      if (lane == 0) {
-        if (a.mean) a.mean[row] = mean[r];
-        if (a.rstd) a.rstd[row] = rstd;
+    for (int r = 0; r < R; ++r) var[r] = rsqrtf(fmaf(var[r], inv_d, a.eps));  // now rstd
+    if (a.mean && l.lane == 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (row0 + r < rows) {
+          a.mean[row0 + r] = mean[r];
+          a.rstd[row0 + r] = var[r];
+        }
+    }
+    TO* po[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) po[r] = out + row_offset(a.os, row0 + r, a.map, D);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if (!l.act[c]) continue;
+      const int col = l.col(c);
+      Pack<float, VEC> wc, bc;
+      if constexpr (LPR) {
+        if constexpr (VEC == 8) {
+          const Pack<float, 4> w0 = load_pack<float, 4>(wb + col), w1 = load_pack<float, 4>(wb + col + 4);
+          const Pack<float, 4> b0 = load_pack<float, 4>(wb + wb_pad + col), b1 = load_pack<float, 4>(wb + wb_pad + col + 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) wc.v[k] = w0.v[k], wc.v[k + 4] = w1.v[k], bc.v[k] = b0.v[k], bc.v[k + 4] = b1.v[k];
+        } else {
+          wc = load_pack<float, VEC>(wb + col);
+          bc = load_pack<float, VEC>(wb + wb_pad + col);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) wc.v[k] = w[c * VEC + k], bc.v[k] = b[c * VEC + k];
       }
-      TO* p = out + row_offset(a.os, row, idx[r], D);
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        if (!act[c]) continue;
+      for (int r = 0; r < R; ++r) {
+        if (row0 + r >= rows) continue;
         Pack<TO, VEC> h;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const int i = c * VEC + v;
-          h.v[v] = from_f32<TO>(fmaf(x[r][i] * rstd, w[i], b[i]));
-        }
-        store_pack(p + (lane + c * width) * VEC, h);
+        for (int k = 0; k < VEC; ++k) h.v[k] = from_f32<TO>(fmaf(x[r][c * VEC + k] * var[r], wc.v[k], bc.v[k]));
+        store_pack(po[r] + col, h);
       }
     }
+    s = s == S - 1 ? 0 : s + 1;
   }
+  copy_wait<0>();
 }
 
-template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, bool HASY>
-cudaError_t launch_one(const NormFwdArgs& a, int threads, cudaStream_t st) {
-  auto kernel = norm_fwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, HASY>;
-  const int per_cta = (LPR ? threads / (LPR ? LPR : 1) : 1) * R;
-  const long long need = ((long long)a.map.rows + per_cta - 1) / per_cta;
-  const long long cap = (long long)device_sm_count() * (2048 / threads);
-  kernel<<<(unsigned)(need < cap ? need : cap), threads, 0, st>>>(a);
-  return cudaGetLastError();
+template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY>
+cudaError_t launch_one(const NormFwdArgs& a, int width, int threads, cudaStream_t st) {
+  static KernelInfo info;
+  const int groups = threads / width, wb = LPR ? ((a.dim + VEC - 1) / VEC * VEC * 8 + 15) / 16 * 16 : 0;
+  const size_t smem = wb + (size_t)groups * S * stage_bytes<TX, TY, VEC, NCH, R, HASY>(width, a.dim);
+  return launch_rows(info, norm_fwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY>, a, width, groups * R, threads, smem, 8, st,
+                     nullptr);
 }
 
-// Lanes per row by the row's number of accesses C = ceil(dim / VEC): the fewest that keep a lane's share
-// within 16 elements (registers), and no more than C rounded up to a power of two below one warp.
 template <class TX, class TY, class TO, int VEC, bool HASY>
 cudaError_t launch_vec(const NormFwdArgs& a, cudaStream_t st) {
-  constexpr int M = 16 / VEC;  // accesses per lane at most
   const int C = (a.dim + VEC - 1) / VEC;
+  constexpr int W = sizeof(TX) == 4 || HASY ? 2 : 4;  // rows of a batch: 16 to 64 bytes a lane and stage
   if constexpr (VEC > 1) {
-    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, 4, HASY>(a, 256, st);
-    if (C <= 16) return launch_one<TX, TY, TO, VEC, 16, 1, 4, HASY>(a, 256, st);
-    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, VEC == 4 ? 4 : 2, HASY>(a, 256, st);
-    if (C <= 64) return launch_one<TX, TY, TO, VEC, 32, 2, VEC == 4 ? 2 : 1, HASY>(a, 256, st);
-    if constexpr (VEC == 4)
-      if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, HASY>(a, 256, st);
+    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, W, 3, HASY>(a, 8, 256, st);
+    if (C <= 16) return launch_one<TX, TY, TO, VEC, 16, 1, W, 3, HASY>(a, 16, 256, st);
+    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, W, 3, HASY>(a, 32, 256, st);
+    if (C <= 64) return launch_one<TX, TY, TO, VEC, 32, 2, W / 2, 3, HASY>(a, 32, 256, st);
+    if constexpr (VEC == 4) {
+      if (C <= 96) return launch_one<TX, TY, TO, VEC, 32, 3, 1, 3, HASY>(a, 32, 256, st);
+      if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, 3, HASY>(a, 32, 256, st);
+    }
   } else {
-    if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 2, HASY>(a, 256, st);
-    if (C <= 512) return launch_one<TX, TY, TO, VEC, 32, 16, 1, HASY>(a, 256, st);
+    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, 2, 3, HASY>(a, 8, 256, st);
+    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, 2, 3, HASY>(a, 32, 256, st);
+    if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, 3, HASY>(a, 32, 256, st);
+    if (C <= 512) return launch_one<TX, TY, TO, VEC, 32, 16, 1, 3, HASY>(a, 32, 256, st);
   }
-  const int threads = ((C + M - 1) / M + 31) / 32 * 32;
-  return launch_one<TX, TY, TO, VEC, 0, M, 1, HASY>(a, threads, st);
+  const RowWidth w = row_width<VEC>(C);
+  if constexpr (VEC == 4)
+    if (w.pieces == 3) return launch_one<TX, TY, TO, VEC, 0, 3, 1, 3, HASY>(a, w.width, w.threads, st);
+  return launch_one<TX, TY, TO, VEC, 0, 16 / VEC, 1, 3, HASY>(a, w.width, w.threads, st);
 }
 
 template <class TX, class TY, class TO, bool HASY>
 cudaError_t launch_types(const NormFwdArgs& a, int vec, cudaStream_t st) {
-  constexpr int FULL = sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2 ? 8 : 4;
-  if (vec >= FULL) return launch_vec<TX, TY, TO, FULL, HASY>(a, st);
+  if constexpr (sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2) {
+    if (vec == 8) return launch_vec<TX, TY, TO, 8, HASY>(a, st);
+  }
+  if (vec >= 4) return launch_vec<TX, TY, TO, 4, HASY>(a, st);
   return launch_vec<TX, TY, TO, 1, HASY>(a, st);
 }
 
