@@ -14,6 +14,7 @@
 
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "triattn_internal.cuh"
 
@@ -175,6 +176,69 @@ __device__ __forceinline__ float load_param(const void* p, int dtype, int i, flo
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
+// ---- two fp32 values a register pair: one instruction does both --------------------------------------
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ Pair both(float v) { return pair(v, v); }
+__device__ __forceinline__ float2 halves(Pair a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float total(Pair a) {
+  const float2 h = halves(a);
+  return h.x + h.y;
+}
+// two neighbouring elements of type T
+template <class T>
+__device__ __forceinline__ Pair to_pair(const T* p) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    uint32_t u;
+    __builtin_memcpy(&u, p, 4);
+    return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
+    return pair(f.x, f.y);
+  } else {
+    return pair(p[0], p[1]);
+  }
+}
+template <class T>
+__device__ __forceinline__ void from_pair(Pair a, T* p) {
+  const float2 h = halves(a);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(h.x, h.y);
+    __builtin_memcpy(p, &r, 4);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 r = __floats2half2_rn(h.x, h.y);
+    __builtin_memcpy(p, &r, 4);
+  } else {
+    p[0] = h.x;
+    p[1] = h.y;
+  }
+}
+
 // ---- rows on their way to a lane ------------------------------------------------------------------------
 // Every lane brings its own share of its next rows into shared memory with asynchronous copies, kStages
 // batches deep, and reads it back when its turn comes.  What is in flight then costs no registers (an SM
@@ -193,6 +257,13 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copy_async_part(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+template <int BYTES>
+__device__ __forceinline__ void copy_zero(uint32_t dst, const void* any) {  // `any` is not read
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, 0;" ::"r"(dst), "l"(any) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, 0;" ::"r"(dst), "l"(any), "n"(BYTES) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() {
@@ -202,21 +273,28 @@ __device__ __forceinline__ void copy_wait() {
 // How a row of dim channels lies on its lanes: LPR lanes of one warp (8, 16 or 32), or with LPR = 0 `width`
 // lanes of several warps, each with NCH pieces of VEC consecutive channels, piece c at channel
 // (lane + c * width) * VEC.  A CTA holds several such groups.
-// VEC > 1: a piece is copied by its own lane.  VEC = 1, for rows that start anywhere (an odd dim, an odd
-// stride or address): the row's lanes copy the 16-byte blocks that hold it, so what a lane reads was
-// copied by its neighbours, and a barrier of the row's lanes (sync) stands before and after the reading.
+// VEC > 1: a piece is copied by its own lane.  All pieces but the last are there on every lane; where the last is
+// not, its place in shared memory holds zeros.
+// VEC = 1, for rows that start anywhere (an odd dim, an odd stride or address): the row's lanes copy the
+// 16-byte blocks that hold it, so what a lane reads was copied by its neighbours, and a barrier of the
+// row's lanes (sync) stands before and after the reading.
 constexpr int RES_MAX_WARPS = 16;  // of a CTA
+constexpr int RES_MAX_GROUPS = 8;  // of several warps, in a CTA
+constexpr int RES_MAX_SUMS = 4;    // of one call
 template <int VEC, int LPR, int NCH>
 struct Lanes {
+  static constexpr int EPL = VEC * NCH, PAIRS = (EPL + 1) / 2;  // channels of a lane, and the pairs that hold them
   int width, lane, group, groups, dim;
-  bool act[NCH];
+  bool last;  // the last piece is there
   __device__ __forceinline__ Lanes(int d, int w) : dim(d) {
     width = LPR ? LPR : w;
     group = threadIdx.x / width;
     lane = threadIdx.x - group * width;
     groups = blockDim.x / width;
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) act[c] = col(c) < dim;
+    last = col(NCH - 1) < dim;
+  }
+  __device__ __forceinline__ bool act(int c) const {
+    return VEC > 1 ? (c < NCH - 1 || last) : col(c) < dim;
   }
   __device__ __forceinline__ int col(int c) const { return (lane + c * width) * VEC; }
   __device__ __forceinline__ void barrier() const {  // of the row's lanes
@@ -230,7 +308,14 @@ struct Lanes {
   }
   // Sums over the row's lanes.  Several warps: one barrier per call; consecutive calls use the two halves
   // of red in turn, and a warp reaches the same half again only after the barrier in between.
-  static constexpr int red_floats = LPR ? 1 : RES_MAX_WARPS * 2 * 2;
+  static constexpr int red_floats = LPR ? 4 : 2 * RES_MAX_SUMS * RES_MAX_GROUPS * RES_MAX_WARPS;
+  // what sum() reads beyond a group's warps: zeros
+  __device__ __forceinline__ void clear(float* red) const {
+    if constexpr (LPR == 0) {
+      for (int i = threadIdx.x; i < red_floats; i += blockDim.x) red[i] = 0.0f;
+      __syncthreads();
+    }
+  }
   template <int K>
   __device__ __forceinline__ void sum(float (&v)[K], float* red, int& phase) const {
     constexpr int W = LPR ? LPR : 32;
@@ -240,38 +325,49 @@ struct Lanes {
       for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     }
     if constexpr (LPR == 0) {
-      static_assert(K <= 2, "");
-      float* s = red + phase * RES_MAX_WARPS * 2;
+      static_assert(K <= RES_MAX_SUMS, "");
+      float* s = red + (phase * RES_MAX_GROUPS + group) * RES_MAX_SUMS * RES_MAX_WARPS;
       phase ^= 1;
-      const int wl = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = width >> 5, first = group * warps;
-      if (wl == 0) {
+      const int warps = width >> 5;
+      if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) s[k * RES_MAX_WARPS + warp] = v[k];
+        for (int k = 0; k < K; ++k) s[k * RES_MAX_WARPS + (lane >> 5)] = v[k];
       }
       barrier();
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        v[k] = wl < warps ? s[k * RES_MAX_WARPS + first + wl] : 0.0f;
+        v[k] = 0.0f;
 #pragma unroll
-        for (int o = RES_MAX_WARPS / 2; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-        v[k] = __shfl_sync(0xffffffffu, v[k], 0);
+        for (int i = 0; i < RES_MAX_WARPS; i += 4) {
+          if (i < warps) {
+            const float4 f = *reinterpret_cast<const float4*>(s + k * RES_MAX_WARPS + i);
+            v[k] += (f.x + f.y) + (f.z + f.w);
+          }
+        }
       }
     }
   }
 };
 
-// Rows of several warps: C pieces (of VEC channels) on `width` lanes, 16 channels a lane at most (registers).
-// fp32 rows take three pieces a lane instead of four where that leaves fewer lanes idle (dim 768, 1536).
+// Rows of several warps: C pieces (of VEC channels) on `width` lanes, 16 channels a lane at most (registers); the
+// number of pieces a lane that leaves the fewest lanes idle, all but the last full.
 struct RowWidth {
   int pieces, width, threads;
 };
 template <int VEC>
-RowWidth row_width(int C) {
-  const auto lanes = [C](int n) { return ((C + n - 1) / n + 31) / 32 * 32; };
-  int n = 16 / VEC;
-  if (VEC == 4 && lanes(3) * 3 < lanes(4) * 4 && lanes(3) <= 512) n = 3;
-  const int width = lanes(n), groups = width < 256 ? 256 / width : 1;
-  return RowWidth{n, width, width * groups};
+RowWidth row_width(int C, int threads) {  // a CTA of about so many threads
+  RowWidth best{16 / VEC, 512, 512};
+  int cost = 1 << 30;
+  for (int n = 16 / VEC; n >= 2; --n) {
+    const int width = ((C + n - 1) / n + 31) / 32 * 32;
+    if (width > 512 || (VEC > 1 && (n - 1) * width > C)) continue;
+    if (width * n < cost) {
+      cost = width * n;
+      best = RowWidth{n, width, width < threads ? threads / width * width : width};
+    }
+    if (VEC != 4) break;
+  }
+  return best;
 }
 
 // Bytes of shared memory that one row of a tensor takes in one stage, per row's group of lanes.
@@ -280,58 +376,214 @@ __host__ __device__ constexpr int row_slot(int width, int dim) {
   return VEC > 1 ? width * NCH * VEC * (int)sizeof(T) : (dim * (int)sizeof(T) + 15) / 16 * 16 + 16;
 }
 
-// One row of a tensor, copied to `slot` and read back from it.
-template <class T, int VEC, int LPR, int NCH>
-struct RowCopy {
-  using L = Lanes<VEC, LPR, NCH>;
-  __device__ __forceinline__ static void issue(const L& l, uint32_t slot, const T* row) {
-    if constexpr (VEC > 1) {
-      constexpr int B = VEC * sizeof(T);
-#pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        if (l.act[c]) {
-          const uint32_t dst = slot + (l.lane + c * l.width) * B;
-          const T* src = row + l.col(c);
-          if constexpr (B <= 16) {
-            copy_async<B>(dst, src);
-          } else {
-#pragma unroll
-            for (int k = 0; k < B; k += 16) copy_async<16>(dst + k, reinterpret_cast<const char*>(src) + k);
-          }
-        }
+// A tensor's rows.  DENSE: row after row, so that a row's address is one multiply-add; else by strides.
+template <class T, bool DENSE>
+struct RowsOf {
+  char* base;
+  uint32_t pitch;  // bytes of a row (DENSE)
+  int64_t s0, s1, s2;
+  __device__ __forceinline__ RowsOf(const void* p, const Strides3& s, int dim, int lane_elements) {
+    base = static_cast<char*>(const_cast<void*>(p)) + lane_elements * (int)sizeof(T);
+    if constexpr (DENSE) {
+      pitch = dim * (uint32_t)sizeof(T);
     } else {
-      // the block that holds the row's first byte begins at most 15 bytes before it, inside the same
-      // 16-byte block of memory; behind the row's last byte nothing is read
-      const uintptr_t first = reinterpret_cast<uintptr_t>(row), last = first + (uintptr_t)l.dim * sizeof(T);
-      uintptr_t at = (first & ~(uintptr_t)15) + (uintptr_t)l.lane * 16;
-      for (uint32_t dst = slot + l.lane * 16; at < last; at += (uintptr_t)l.width * 16, dst += l.width * 16) {
-        const int n = last - at < 16 ? (int)(last - at) : 16;
-        copy_async_part(dst, reinterpret_cast<const void*>(at), n);
-      }
+      s0 = s.s[0] * (int)sizeof(T);
+      s1 = s.s[1] * (int)sizeof(T);
+      s2 = s.s[2] * (int)sizeof(T);
     }
   }
-  // piece c, as floats
-  __device__ __forceinline__ static void read(const L& l, const char* slot, const T* row, int c, float (&v)[VEC]) {
-    if constexpr (VEC > 1) {
-      const Pack<T, VEC> p = load_pack<T, VEC>(reinterpret_cast<const T*>(slot) + (l.lane + c * l.width) * VEC);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = to_f32(p.v[k]);
+  __device__ __forceinline__ T* at(uint32_t row, const RowMap& map) const {
+    if constexpr (DENSE) {
+      return reinterpret_cast<T*>(base + (uint64_t)row * pitch);
     } else {
-      v[0] = to_f32(reinterpret_cast<const T*>(slot + (reinterpret_cast<uintptr_t>(row) & 15))[l.col(c)]);
+      const RowIndex i = map.at(row);
+      return reinterpret_cast<T*>(base + s0 * i.i0 + s1 * i.i1 + s2 * i.i2);
     }
   }
 };
 
-// Keep bits of the NCH pieces of a lane: bit k of keep[c].  pos0: position of the row's first channel.
-template <int VEC, int LPR, int NCH>
-__device__ __forceinline__ void keep_pieces(const Lanes<VEC, LPR, NCH>& l, const Philox& rng, uint64_t pos0,
-                                            uint32_t drop_max, uint32_t (&keep)[NCH]) {
+// An input's rows on their way through shared memory: copied to a slot and read back from it.  `off` is the
+// slot's place in the group's ring.
+template <class T, int VEC, int LPR, int NCH, bool DENSE>
+struct RowIn {
+  using L = Lanes<VEC, LPR, NCH>;
+  static constexpr int B = VEC * sizeof(T);
+  static_assert(VEC == 1 || B == 8 || B == 16, "");
+  const L& l;
+  const RowMap& map;
+  RowsOf<T, DENSE> rows;
+  char* ring;  // VEC > 1: at the lane's first piece
+  uint32_t ring32;
+  __device__ __forceinline__ RowIn(const L& l_, const RowMap& m, const void* p, const Strides3& s, char* r)
+      : l(l_), map(m), rows(p, s, l_.dim, VEC > 1 ? l_.lane * VEC : 0) {
+    ring = r + (VEC > 1 ? l.lane * B : 0);
+    ring32 = smem_u32(ring);
+  }
+  __device__ __forceinline__ int step() const { return l.width * B; }  // between pieces
+  // zeros where a lane has no last piece, once for every slot
+  __device__ __forceinline__ void clear(int off) const {
+    if constexpr (VEC > 1) {
+      if (!l.last) {
+        uint64_t* p = reinterpret_cast<uint64_t*>(ring + off + (NCH - 1) * step());
+#pragma unroll
+        for (int k = 0; k < B / 8; ++k) p[k] = 0;
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(int off, uint32_t row) const {
+    const T* p = rows.at(row, map);
+    if constexpr (VEC > 1) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c)
+        if (l.act(c)) copy_async<B>(ring32 + off + c * step(), reinterpret_cast<const char*>(p) + c * step());
+    } else {
+      // the block that holds the row's first byte begins at most 15 bytes before it, inside the same
+      // 16-byte block of memory; behind the row's last byte nothing is read
+      const uintptr_t first = reinterpret_cast<uintptr_t>(p), end = first + (uintptr_t)l.dim * sizeof(T);
+      uintptr_t at = (first & ~(uintptr_t)15) + (uintptr_t)l.lane * 16;
+      for (uint32_t dst = ring32 + off + l.lane * 16; at < end; at += (uintptr_t)l.width * 16, dst += l.width * 16)
+        copy_async_part(dst, reinterpret_cast<const void*>(at), end - at < 16 ? (int)(end - at) : 16);
+    }
+  }
+  // a row that is not there: zeros (VEC > 1; elsewhere read() takes care of it)
+  __device__ __forceinline__ void issue_none(int off) const {
+    if constexpr (VEC > 1) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) copy_zero<B>(ring32 + off + c * step(), rows.base);
+    }
+  }
+  __device__ __forceinline__ void read(int off, uint32_t row, bool live, Pair (&x)[L::PAIRS]) const {
+    if constexpr (VEC > 1) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const Pack<T, VEC> p = load_pack<T, VEC>(reinterpret_cast<const T*>(ring + off + c * step()));
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) x[c * VEC / 2 + j] = to_pair(p.v + 2 * j);
+      }
+    } else {
+      const T* p = reinterpret_cast<const T*>(ring + off + (reinterpret_cast<uintptr_t>(rows.at(row, map)) & 15));
+      float v[2 * L::PAIRS];
+#pragma unroll
+      for (int c = 0; c < 2 * L::PAIRS; ++c) v[c] = c < NCH && live && l.act(c) ? to_f32(p[l.col(c)]) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < L::PAIRS; ++j) x[j] = pair(v[2 * j], v[2 * j + 1]);
+    }
+  }
+};
+// An output's rows.
+template <class T, int VEC, int LPR, int NCH, bool DENSE>
+struct RowOut {
+  using L = Lanes<VEC, LPR, NCH>;
+  const L& l;
+  const RowMap& map;
+  RowsOf<T, DENSE> rows;
+  __device__ __forceinline__ RowOut(const L& l_, const RowMap& m, const void* p, const Strides3& s)
+      : l(l_), map(m), rows(p, s, l_.dim, l_.lane * VEC) {}
+  __device__ __forceinline__ T* at(uint32_t row) const { return rows.at(row, map); }
+  // piece c of a row's values, if the lane has it; p = at(row)
+  __device__ __forceinline__ void piece(T* p, int c, const Pair (&x)[L::PAIRS]) const {
+    if (!l.act(c)) return;
+    if constexpr (VEC > 1) {
+      Pack<T, VEC> o;
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) from_pair(x[c * VEC / 2 + j], o.v + 2 * j);
+      store_pack(p + c * l.width * VEC, o);
+    } else {
+      const float2 h = halves(x[c / 2]);
+      p[c * l.width] = from_f32<T>(c & 1 ? h.y : h.x);
+    }
+  }
+  __device__ __forceinline__ void row(uint32_t row, const Pair (&x)[L::PAIRS]) const {
+    T* p = at(row);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) piece(p, c, x);
+  }
+};
+
+// a lane's channels of a LayerNorm parameter; zero where it has none
+template <class T, int VEC, int LPR, int NCH, int P>
+__device__ __forceinline__ void load_pairs_of(const Lanes<VEC, LPR, NCH>& l, const T* p, Pair (&x)[P]) {
+  if (VEC > 1 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0) {
+    Pack<T, 4> v[(VEC * NCH + 3) / 4];  // all on their way before the first is used
+#pragma unroll
+    for (int q = 0; q < VEC * NCH / 4; ++q)
+      if (l.act(q * 4 / VEC)) v[q] = load_pack<T, 4>(p + l.col(q * 4 / VEC) + q * 4 % VEC);
+#pragma unroll
+    for (int q = 0; q < VEC * NCH / 4; ++q) {
+      const bool a = l.act(q * 4 / VEC);
+      x[2 * q] = a ? to_pair(v[q].v) : both(0.0f);
+      x[2 * q + 1] = a ? to_pair(v[q].v + 2) : both(0.0f);
+    }
+  } else {
+    float v[2 * P];
+#pragma unroll
+    for (int i = 0; i < 2 * P; ++i)
+      v[i] = i < VEC * NCH && l.act(i / VEC) ? to_f32(p[l.col(i / VEC) + i % VEC]) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < P; ++j) x[j] = pair(v[2 * j], v[2 * j + 1]);
+  }
+}
+template <int VEC, int LPR, int NCH, int P>
+__device__ __forceinline__ void load_pairs(const Lanes<VEC, LPR, NCH>& l, const void* p, int dtype, float absent, Pair (&x)[P]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      x[j] = pair(2 * j < VEC * NCH && l.act(2 * j / VEC) ? absent : 0.0f,
+                  2 * j + 1 < VEC * NCH && l.act((2 * j + 1) / VEC) ? absent : 0.0f);
+  } else if (dtype == DT_F32) {
+    load_pairs_of(l, static_cast<const float*>(p), x);
+  } else if (dtype == DT_F16) {
+    load_pairs_of(l, static_cast<const __half*>(p), x);
+  } else {
+    load_pairs_of(l, static_cast<const __nv_bfloat16*>(p), x);
+  }
+}
+// x += m on the channels that are there, and t += x * x
+template <int VEC, int LPR, int NCH, int P>
+__device__ __forceinline__ void centre(const Lanes<VEC, LPR, NCH>& l, Pair m, Pair (&x)[P], Pair& t) {
+  if constexpr (VEC > 1) {
+    constexpr int N = VEC / 2;
+#pragma unroll
+    for (int j = 0; j < P - N; ++j) {
+      x[j] = x[j] + m;
+      t = fma2(x[j], x[j], t);
+    }
+    if (l.last) {
+#pragma unroll
+      for (int j = P - N; j < P; ++j) {
+        x[j] = x[j] + m;
+        t = fma2(x[j], x[j], t);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const float2 a = halves(x[j]), d = halves(x[j] + m);
+      x[j] = pair(l.act(2 * j) ? d.x : a.x, 2 * j + 1 < NCH && l.act(2 * j + 1) ? d.y : a.y);
+      t = fma2(x[j], x[j], t);
+    }
+  }
+}
+
+// f(kept, i) for a lane's channels i = 0 .. EPL - 1, drawn at the positions from pos0 (the row's first) on.
+template <int VEC, int LPR, int NCH, class F>
+__device__ __forceinline__ void each_kept(const Lanes<VEC, LPR, NCH>& l, const Philox& rng, uint64_t pos0,
+                                          uint32_t drop_max, F&& f) {
   if constexpr (VEC > 1) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) keep[c] = keep_bits<VEC>(rng, pos0 + l.col(c), drop_max);
+    for (int c = 0; c < NCH; ++c) {
+#pragma unroll
+      for (int q = 0; q < VEC; q += 4) {
+        const uint4 w = rng.block((pos0 + l.col(c) + q) >> 2);
+        f(w.x > drop_max, c * VEC + q);
+        f(w.y > drop_max, c * VEC + q + 1);
+        f(w.z > drop_max, c * VEC + q + 2);
+        f(w.w > drop_max, c * VEC + q + 3);
+      }
+    }
   } else if constexpr (NCH < 3) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) keep[c] = keep_bits<1>(rng, pos0 + l.col(c), drop_max);
+    for (int c = 0; c < NCH; ++c) f(rng.word(pos0 + l.col(c)) > drop_max, c);
   } else {
     // The 32 channels of a warp's piece lie in at most 9 blocks of four positions: lanes 0..8, 9..17 and
     // 18..26 draw those of three pieces at a time, and every lane fetches its bit.
@@ -339,14 +591,13 @@ __device__ __forceinline__ void keep_pieces(const Lanes<VEC, LPR, NCH>& l, const
     const int warp0 = l.lane - wl;  // first channel of the warp in piece 0
 #pragma unroll
     for (int c = 0; c < NCH; c += 3) {
-      const uint64_t mine = pos0 + warp0 + (c + third) * l.width;
-      const uint32_t bits = keep_bits<4>(rng, ((mine >> 2) + block) << 2, drop_max);
+      const uint64_t mine = (pos0 + warp0 + (c + third) * l.width) >> 2;
+      const uint32_t bits = keep_bits<4>(rng, (mine + block) << 2, drop_max);
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
         if (c + j < NCH) {
-          const uint32_t at = (uint32_t)(pos0 + warp0 + (c + j) * l.width) & 3;  // in the first block
-          const uint32_t b = __shfl_sync(0xffffffffu, bits, j * 9 + ((at + wl) >> 2));
-          keep[c + j] = b >> ((at + wl) & 3) & 1;
+          const uint32_t at = ((uint32_t)(pos0 + warp0 + (c + j) * l.width) & 3) + wl;  // from the first block on
+          f(__shfl_sync(0xffffffffu, bits, j * 9 + (at >> 2)) >> (at & 3) & 1, c + j);
         }
       }
     }
@@ -394,44 +645,49 @@ struct DropoutAddArgs {
   Dropout drop;
 };
 
-// A persistent launch over rows: as many CTAs as fit on the GPU at once, `most` per SM at most, or as the rows
-// need (per_cta rows each per sweep).  What a kernel needs to be known for that is asked for once per device.
+// How the batches of a launch (groups * R rows each) are shared out: the first `big` CTAs take `many` batches
+// each, the others `few`.
+struct Split {
+  uint32_t big, many, few, batches;
+  __device__ __forceinline__ void range(uint32_t cta, uint32_t& first, uint32_t& end) const {
+    first = cta < big ? cta * many : big * many + (cta - big) * few;
+    end = first + (cta < big ? many : few);
+    if (end > batches) end = batches;
+  }
+};
+
+// What a kernel needs to be known for its launches, asked for once per device.
 struct KernelInfo {
   std::mutex mu;
   int regs[64] = {0};
-};
-template <class Kernel, class Args>
-cudaError_t launch_rows(KernelInfo& info, Kernel kernel, const Args& a, int width, int per_cta, int threads, size_t smem,
-                        int most, cudaStream_t st, unsigned* ctas) {
-  constexpr int kSmem = 227 * 1024, kStatic = 1024;  // of an SM; a CTA's static and reserved share, rounded up
-  int dev = 0, regs = 0;
-  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lk(info.mu);
-    if (!info.regs[dev]) {
-      cudaFuncAttributes f;
-      if (cudaError_t e = cudaFuncGetAttributes(&f, kernel); e != cudaSuccess) return e;
-      if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kSmem - (int)f.sharedSizeBytes);
-          e != cudaSuccess)
-        return e;
-      info.regs[dev] = f.numRegs;
+  // CTAs of a launch that fit on an SM at once
+  template <class Kernel>
+  cudaError_t fit(Kernel kernel, int threads, size_t smem, int* ctas) {
+    constexpr int kSmem = 227 * 1024, kReserved = 1024;  // of an SM; a CTA's own share beside its dynamic one
+    int dev = 0, r = 0, fixed = 2048;
+    if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    {
+      std::lock_guard<std::mutex> lk(mu);
+      if (!regs[dev]) {
+        cudaFuncAttributes f;
+        if (cudaError_t e = cudaFuncGetAttributes(&f, kernel); e != cudaSuccess) return e;
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kSmem - (int)f.sharedSizeBytes);
+            e != cudaSuccess)
+          return e;
+        regs[dev] = f.numRegs;
+      }
+      r = regs[dev];
     }
-    regs = info.regs[dev];
+    const int warps = threads / 32;
+    int n = 65536 / ((r + 7) / 8 * 8 * 32 * warps);
+    if (n > 64 / warps) n = 64 / warps;
+    if (n > (int)(kSmem / (smem + kReserved + fixed))) n = (int)(kSmem / (smem + kReserved + fixed));
+    *ctas = n < 1 ? 1 : n;
+    return cudaSuccess;
   }
-  const int warps = threads / 32;
-  int fit = 65536 / ((regs + 7) / 8 * 8 * 32 * warps);
-  if (fit > 64 / warps) fit = 64 / warps;
-  if (fit > (int)(kSmem / (smem + 2 * kStatic))) fit = (int)(kSmem / (smem + 2 * kStatic));
-  if (fit < 1) fit = 1;
-  if (fit > most) fit = most;
-  const long long need = ((long long)a.map.rows + per_cta - 1) / per_cta, cap = (long long)device_sm_count() * fit;
-  const unsigned grid = (unsigned)(need < cap ? need : cap);
-  if (ctas) *ctas = grid;
-  kernel<<<grid, threads, smem, st>>>(a, width);
-  return cudaGetLastError();
-}
+};
 
 // what every tensor of a call allows: elements moved at a time (8, 4 or 1)
 cudaError_t launch_norm_fwd(const NormFwdArgs& a, int z_dtype, int y_dtype, int out_dtype, int vec, cudaStream_t st);

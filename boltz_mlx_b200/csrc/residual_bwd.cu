@@ -9,65 +9,74 @@
 // registers until the CTA has seen its last row; they are then joined in shared memory, written as one
 // partial row per CTA and summed by a second small kernel in the order of the CTAs: no atomics, the same
 // bits on every run.
+#include <cooperative_groups.h>
+
 #include "residual.cuh"
 
 namespace triattn {
 namespace {
 
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 4;   // resident at most
+constexpr int kPartials = 5;   // CTAs of a launch at most, times those
 
 template <class TX, class TO, int VEC, int NCH, int R, bool HASY>
 constexpr int stage_bytes(int width, int dim) {
   return R * ((HASY ? 2 : 1) * row_slot<TX, VEC, NCH>(width, dim) + row_slot<TO, VEC, NCH>(width, dim));
 }
 
-template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY>
-__global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwdArgs a, int width) {
-  constexpr int EPL = VEC * NCH;
-  extern __shared__ __align__(16) char smem[];  // the groups' stages; at the end [groups][2][dim] column sums
+template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY, bool DENSE>
+__global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwdArgs a, int width, Split split) {
   using L = Lanes<VEC, LPR, NCH>;
-  __shared__ float red[L::red_floats];
+  constexpr int P = L::PAIRS;
+  extern __shared__ __align__(16) char smem[];  // the groups' stages; at the end [groups][2][dim] column sums
+  __shared__ __align__(16) float red[L::red_floats];
   int phase = 0;
   const L l(a.dim, width);
-  using CX = RowCopy<TX, VEC, LPR, NCH>;
-  using CO = RowCopy<TO, VEC, LPR, NCH>;
   const int D = a.dim;
   const float inv_d = 1.0f / (float)D;
-  const TX* x = static_cast<const TX*>(a.x);
-  const TX* ds = static_cast<const TX*>(a.ds);
-  const TO* dout = static_cast<const TO*>(a.dout);
-  TX* dx = static_cast<TX*>(a.dx);
-  TY* dy = static_cast<TY*>(a.dy);
 
-  float w[EPL], dw[EPL], db[EPL];
+  Pair w[P], dw[P], db[P];
+  load_pairs(l, a.weight, a.param_dtype, 1.0f, w);
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    w[i] = l.act[i / VEC] ? load_param(a.weight, a.param_dtype, l.col(i / VEC) + i % VEC, 1.0f) : 0.0f;
-    dw[i] = db[i] = 0.0f;
-  }
+  for (int j = 0; j < P; ++j) dw[j] = db[j] = both(0.0f);
+  l.clear(red);
   const Philox rng(a.drop);
-  const bool has_ds = HASY && ds, has_dy = HASY && dy;
+  const bool has_ds = HASY && a.ds, has_dy = HASY && a.dy;
   const bool row_draw = has_dy && a.drop.on && !a.drop.per_channel, draw = has_dy && a.drop.on && a.drop.per_channel;
 
   const int slot_x = row_slot<TX, VEC, NCH>(l.width, D), slot_o = row_slot<TO, VEC, NCH>(l.width, D);
   const int stage = stage_bytes<TX, TO, VEC, NCH, R, HASY>(l.width, D);
   char* ring = smem + l.group * S * stage;
-  const uint32_t ring32 = smem_u32(ring);
+  const RowIn<TX, VEC, LPR, NCH, DENSE> x(l, a.map, a.x, a.xs, ring), ds(l, a.map, a.ds, a.dss, ring + R * (slot_x + slot_o));
+  const RowIn<TO, VEC, LPR, NCH, DENSE> dout(l, a.map, a.dout, a.dos, ring + R * slot_x);
+  const RowOut<TX, VEC, LPR, NCH, true> dx(l, a.map, a.dx, a.xs);
+  const RowOut<TY, VEC, LPR, NCH, true> dy(l, a.map, a.dy, a.xs);
+  for (int k = 0; k < S; ++k) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      x.clear(k * stage + r * slot_x);
+      dout.clear(k * stage + r * slot_o);
+      if (HASY) ds.clear(k * stage + r * slot_x);
+    }
+  }
 
-  const uint32_t rows = a.map.rows, step = gridDim.x * l.groups * R;
+  const uint32_t rows = a.map.rows, step = l.groups * R;
   const auto issue = [&](uint32_t base, int s) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint32_t row = base + l.group * R + r;
-      if (row >= rows) continue;
-      const uint32_t at = ring32 + s * stage;
-      CX::issue(l, at + r * slot_x, x + row_offset(a.xs, row, a.map, D));
-      CO::issue(l, at + R * slot_x + r * slot_o, dout + row_offset(a.dos, row, a.map, D));
+      if (row >= rows) {  // adds nothing to the column sums
+        x.issue_none(s * stage + r * slot_x);
+        dout.issue_none(s * stage + r * slot_o);
+        continue;
+      }
+      x.issue(s * stage + r * slot_x, row);
+      dout.issue(s * stage + r * slot_o, row);
       if constexpr (HASY)
-        if (has_ds) CX::issue(l, at + R * (slot_x + slot_o) + r * slot_x, ds + row_offset(a.dss, row, a.map, D));
+        if (has_ds) ds.issue(s * stage + r * slot_x, row);
     }
   };
-  float mean[R], rstd[R], mean_next[R], rstd_next[R];  // of the batch in hand and of the next one
+  float mean_next[R], rstd_next[R];  // of the next batch
   const auto statistics = [&](uint32_t base) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -77,17 +86,22 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     }
   };
 
-  uint32_t ahead = blockIdx.x * l.groups * R;
+  uint32_t first, end;  // rows of this CTA
+  split.range(blockIdx.x, first, end);
+  first *= step;
+  end *= step;
+  uint32_t ahead = first;
   statistics(ahead);
 #pragma unroll
   for (int s = 0; s < S - 1; ++s, ahead += step) {
-    if (ahead < rows) issue(ahead, s);
+    if (ahead < end) issue(ahead, s);
     copy_commit();
   }
   int s = 0;
-  for (uint32_t base = blockIdx.x * l.groups * R; base < rows; base += step, ahead += step) {
-    if (ahead < rows) issue(ahead, s == 0 ? S - 1 : s - 1);
+  for (uint32_t base = first; base < end; base += step, ahead += step) {
+    if (ahead < end) issue(ahead, s == 0 ? S - 1 : s - 1);
     copy_commit();
+    float mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       mean[r] = mean_next[r];
@@ -97,50 +111,40 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     copy_wait<S - 1>();
     l.sync();
     const uint32_t row0 = base + l.group * R;
-    const char* here = ring + s * stage;
     // v[2 r] = sum g, v[2 r + 1] = sum g xh
-    float xh[R][EPL], g[R][EPL], v[2 * R];
+    Pair xh[R][P], g[R][P];
+    float v[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint32_t row = row0 + r;
       const bool live = row < rows;
-      const TX* xrow = x + (VEC == 1 ? row_offset(a.xs, row, a.map, D) : 0);
-      const TO* orow = dout + (VEC == 1 ? row_offset(a.dos, row, a.map, D) : 0);
-      v[2 * r] = v[2 * r + 1] = 0.0f;
+      x.read(s * stage + r * slot_x, row, live, xh[r]);
+      dout.read(s * stage + r * slot_o, row, live, g[r]);
+      const Pair q = both(rstd[r]), mq = both(-mean[r] * rstd[r]);
+      Pair s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        float xv[VEC], dv[VEC];
-        const bool in = live && l.act[c];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) xv[k] = mean[r], dv[k] = 0.0f;
-        if (in) {
-          CX::read(l, here + r * slot_x, xrow, c, xv);
-          CO::read(l, here + R * slot_x + r * slot_o, orow, c, dv);
-        }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const int i = c * VEC + k;
-          xh[r][i] = (xv[k] - mean[r]) * rstd[r];
-          dw[i] = fmaf(dv[k], xh[r][i], dw[i]);
-          db[i] += dv[k];
-          g[r][i] = dv[k] * w[i];
-          v[2 * r] += g[r][i];
-          v[2 * r + 1] = fmaf(g[r][i], xh[r][i], v[2 * r + 1]);
-        }
+      for (int j = 0; j < P; ++j) {
+        xh[r][j] = fma2(xh[r][j], q, mq);  // where there is no channel, dout and the weight are zero
+        dw[j] = fma2(g[r][j], xh[r][j], dw[j]);
+        db[j] = db[j] + g[r][j];
+        g[r][j] = g[r][j] * w[j];
+        s1 = s1 + g[r][j];
+        s2 = fma2(g[r][j], xh[r][j], s2);
       }
+      v[2 * r] = total(s1);
+      v[2 * r + 1] = total(s2);
     }
     l.sum(v, red, phase);
     uint32_t whole = ~0u;  // bit r: row r is not dropped whole
     if constexpr (HASY) {
       if (row_draw) {
+        whole = 0;
         if constexpr (LPR && R > 1) {
           const uint32_t row = row0 + (l.lane & (R - 1));
           const bool k = row < rows && rng.word(mask_base(a.drop, a.map.at(row))) > a.drop.drop_max;
-          whole = 0;
 #pragma unroll
           for (int r = 0; r < R; ++r) whole |= __shfl_sync(0xffffffffu, (uint32_t)k, r, LPR) << r;
         } else {
-          whole = 0;
 #pragma unroll
           for (int r = 0; r < R; ++r)
             if (row0 + r < rows && rng.word(mask_base(a.drop, a.map.at(row0 + r))) > a.drop.drop_max) whole |= 1u << r;
@@ -151,43 +155,33 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     for (int r = 0; r < R; ++r) {
       const uint32_t row = row0 + r;
       const bool live = row < rows;
-      const float c1 = v[2 * r] * inv_d, c2 = v[2 * r + 1] * inv_d;
-      uint32_t keep[NCH];
+      const float t = -inv_d * rstd[r];
+      const Pair c1 = both(v[2 * r] * t), c2 = both(v[2 * r + 1] * t), q = both(rstd[r]);
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) keep[c] = whole >> r & 1 ? 0xffu : 0u;
-      if constexpr (HASY)
-        if (draw) keep_pieces(l, rng, mask_base(a.drop, a.map.at(live ? row : rows - 1)), a.drop.drop_max, keep);
-      const TX* srow = ds + (HASY && VEC == 1 && has_ds ? row_offset(a.dss, row, a.map, D) : 0);
+      for (int j = 0; j < P; ++j) g[r][j] = fma2(g[r][j], q, fma2(xh[r][j], c2, c1));
+      if constexpr (HASY) {
+        if (has_ds) {
+          Pair sv[P];
+          ds.read(s * stage + r * slot_x, row, live, sv);
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        if (!live || !l.act[c]) continue;
-        const int col = l.col(c);
-        float f[VEC], sv[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const int i = c * VEC + k;
-          f[k] = rstd[r] * (g[r][i] - c1 - xh[r][i] * c2);
+          for (int j = 0; j < P; ++j) g[r][j] = g[r][j] + sv[j];
         }
-        if constexpr (HASY) {
-          if (has_ds) {
-            CX::read(l, here + R * (slot_x + slot_o) + r * slot_x, srow, c, sv);
+      }
+      if (a.dx && live) dx.row(row, g[r]);
+      if constexpr (HASY) {
+        if (has_dy) {
+          if (draw) {
+            each_kept(l, rng, mask_base(a.drop, a.map.at(live ? row : rows - 1)), a.drop.drop_max, [&](bool k, int i) {
+              const float2 gi = halves(g[r][i / 2]);
+              const float f = k ? (i & 1 ? gi.y : gi.x) * a.drop.scale : 0.0f;
+              g[r][i / 2] = i & 1 ? pair(gi.x, f) : pair(f, gi.y);
+            });
+          } else {
+            const Pair scale = both(a.drop.scale);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) f[k] += sv[k];
+            for (int j = 0; j < P; ++j) g[r][j] = whole >> r & 1 ? g[r][j] * scale : both(0.0f);
           }
-        }
-        if (dx) {
-          Pack<TX, VEC> o;
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) o.v[k] = from_f32<TX>(f[k]);
-          store_pack(dx + (int64_t)row * D + col, o);
-        }
-        if constexpr (HASY) {
-          if (dy) {
-            Pack<TY, VEC> q;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) q.v[k] = from_f32<TY>(keep[c] >> k & 1 ? f[k] * a.drop.scale : 0.0f);
-            store_pack(dy + (int64_t)row * D + col, q);
-          }
+          if (live) dy.row(row, g[r]);
         }
       }
     }
@@ -202,9 +196,9 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
 #pragma unroll
   for (int o = LPR ? LPR : 32; o < 32; o <<= 1) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-      db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+    for (int j = 0; j < P; ++j) {
+      dw[j] = dw[j] + Pair{__shfl_xor_sync(0xffffffffu, dw[j].v, o)};
+      db[j] = db[j] + Pair{__shfl_xor_sync(0xffffffffu, db[j].v, o)};
     }
   }
   const int sets = LPR ? blockDim.x >> 5 : l.groups;
@@ -213,14 +207,12 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
   __syncthreads();  // every warp has read its last rows
   if (writes) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
-      if (l.act[c]) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          mine[l.col(c) + k] = dw[c * VEC + k];
-          mine[D + l.col(c) + k] = db[c * VEC + k];
-        }
-      }
+    for (int i = 0; i < L::EPL; ++i) {
+      if (!l.act(i / VEC)) continue;
+      const float2 u = halves(dw[i / 2]), t = halves(db[i / 2]);
+      mine[l.col(i / VEC) + i % VEC] = i & 1 ? u.y : u.x;
+      mine[D + l.col(i / VEC) + i % VEC] = i & 1 ? t.y : t.x;
+    }
   }
   if (sets == 1) return;
   __syncthreads();
@@ -231,42 +223,82 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
   }
 }
 
-// Column sums of the CTAs' partial rows: 32 columns per CTA, 16 warps over the partial rows.
+// Column sums of the CTAs' partial rows: a cluster of kJoin CTAs for 32 columns, each of its warps with every
+// 16 * kJoin-th row; the cluster's first CTA adds up what the others hold in their shared memory.  One CTA
+// alone needs 15 us for the 2000 partial rows of a long launch, the cluster 3.
+constexpr int kJoin = 8;
 template <class TP>
-__global__ void __launch_bounds__(512) norm_bwd_join_kernel(const float* __restrict__ partial, int ctas, int dim,
-                                                            TP* __restrict__ dweight, TP* __restrict__ dbias) {
+__global__ void __cluster_dims__(kJoin, 1, 1) __launch_bounds__(512)
+    norm_bwd_join_kernel(const float* __restrict__ partial, int ctas, int dim, TP* __restrict__ dweight,
+                         TP* __restrict__ dbias) {
+  namespace cg = cooperative_groups;
   __shared__ float part[16][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + lane;  // of 2 * dim
+  __shared__ float sum[32];
+  const auto cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = blockIdx.x / kJoin * 32 + lane;  // of 2 * dim
   float s = 0.0f;
-  if (col < 2 * dim)
-    for (int i = warp; i < ctas; i += 16) s += partial[(size_t)i * 2 * dim + col];
+  if (col < 2 * dim) {
+#pragma unroll 8
+    for (int i = rank * 16 + warp; i < ctas; i += 16 * kJoin) s += partial[(size_t)i * 2 * dim + col];
+  }
   part[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && col < 2 * dim) {
+  if (warp == 0) {
     s = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += part[i][lane];
+    sum[lane] = s;
+  }
+  cluster.sync();
+  if (rank == 0 && warp == 0 && col < 2 * dim) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) s += *cluster.map_shared_rank(&sum[lane], i);
     if (col < dim) {
       if (dweight) dweight[col] = from_f32<TP>(s);
     } else if (dbias) {
       dbias[col - dim] = from_f32<TP>(s);
     }
   }
+  cluster.sync();  // no CTA leaves while its sums are read
 }
 
-template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY>
+// Three quarters of the batches go to the CTAs that are resident from the start, in equal shares; the rest in
+// shares an eighth as large, to whichever SM comes free: equal shares alone leave the SMs that the memory
+// system serves last working alone at the end.  Every CTA costs a partial row of 16 bytes a channel (written
+// and read), so a share has kRows rows at least, or there is one kind of CTA only.  What a CTA adds up goes by
+// its index, not by when it runs.
+constexpr uint32_t kRows = 64;
+Split share(uint32_t batches, uint32_t resident, uint32_t per) {
+  Split s{resident, batches / 4 * 3 / resident, 0, batches};
+  s.few = s.many / 8;
+  if (s.few * per < kRows) s.few = (kRows + per - 1) / per;
+  if (s.few * 2 > s.many) {
+    s.many = (batches + resident - 1) / resident;
+    s.big = (batches + s.many - 1) / s.many;
+    s.few = 0;
+  }
+  return s;
+}
+
+template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY, bool DENSE>
 cudaError_t launch_one(const NormBwdArgs& a, int width, int threads, cudaStream_t st) {
   static KernelInfo info;
   const int groups = threads / width, sets = LPR ? threads / 32 : groups;
   size_t smem = (size_t)groups * S * stage_bytes<TX, TO, VEC, NCH, R, HASY>(width, a.dim);
   if (const size_t sums = (size_t)sets * 2 * a.dim * 4; sets > 1 && smem < sums) smem = sums;
-  unsigned grid = 0;
-  if (cudaError_t e = launch_rows(info, norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY>, a, width, groups * R, threads,
-                                  smem, kCtasPerSm, st, &grid);
-      e != cudaSuccess || !a.partial)
+  int fit = 0;
+  if (cudaError_t e = info.fit(norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE>, threads, smem, &fit);
+      e != cudaSuccess)
     return e;
-  const int blocks = (2 * a.dim + 31) / 32;
+  if (fit > kCtasPerSm) fit = kCtasPerSm;
+  const uint32_t per = groups * R, batches = ((uint32_t)a.map.rows + per - 1) / per;
+  const Split split = share(batches, (uint32_t)(device_sm_count() * fit), per);
+  const uint32_t grid = split.big + (split.few ? (batches - split.big * split.many + split.few - 1) / split.few : 0);
+  norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE><<<grid, threads, smem, st>>>(a, width, split);
+  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess || !a.partial) return e;
+  const int blocks = (2 * a.dim + 31) / 32 * kJoin;
   if (a.param_dtype == DT_F32)
     norm_bwd_join_kernel<<<blocks, 512, 0, st>>>(a.partial, (int)grid, a.dim, static_cast<float*>(a.dweight),
                                                 static_cast<float*>(a.dbias));
@@ -279,42 +311,49 @@ cudaError_t launch_one(const NormBwdArgs& a, int width, int threads, cudaStream_
   return cudaGetLastError();
 }
 
-template <class TX, class TY, class TO, int VEC, bool HASY>
+template <class TX, class TY, class TO, int VEC, bool HASY, bool DENSE>
 cudaError_t launch_vec(const NormBwdArgs& a, cudaStream_t st) {
   const int C = (a.dim + VEC - 1) / VEC;
+#define LAUNCH(LPR, NCH, R, S, WIDTH, THREADS) \
+  return launch_one<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE>(a, WIDTH, THREADS, st)
   if constexpr (VEC > 1) {
-    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, 2, 3, HASY>(a, 8, 256, st);
-    if (C <= 16) return launch_one<TX, TY, TO, VEC, 16, 1, 2, 3, HASY>(a, 16, 256, st);
-    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, 2, 3, HASY>(a, 32, 256, st);
-    if (C <= 64) return launch_one<TX, TY, TO, VEC, 32, 2, 1, 3, HASY>(a, 32, 256, st);
+    if (C <= 8) LAUNCH(8, 1, 4, 2, 8, 256);
+    if (C <= 16) LAUNCH(16, 1, 4, 2, 16, 256);
+    if (C <= 32) LAUNCH(32, 1, 16 / VEC, 2, 32, 256);
+    if (C <= 64) LAUNCH(32, 2, 2, 2, 32, 256);
     if constexpr (VEC == 4) {
-      if (C <= 96) return launch_one<TX, TY, TO, VEC, 32, 3, 1, 3, HASY>(a, 32, 256, st);
-      if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, 3, HASY>(a, 32, 256, st);
+      if (C <= 96) LAUNCH(32, 3, 1, 3, 32, 256);
+      if (C <= 128) LAUNCH(32, 4, 1, 3, 32, 256);
     }
   } else {
-    if (C <= 8) return launch_one<TX, TY, TO, VEC, 8, 1, 2, 3, HASY>(a, 8, 256, st);
-    if (C <= 32) return launch_one<TX, TY, TO, VEC, 32, 1, 2, 3, HASY>(a, 32, 256, st);
-    if (C <= 128) return launch_one<TX, TY, TO, VEC, 32, 4, 1, 3, HASY>(a, 32, 256, st);
-    if (C <= 512) return launch_one<TX, TY, TO, VEC, 32, 16, 1, 3, HASY>(a, 32, 256, st);
+    if (C <= 8) LAUNCH(8, 1, 2, 3, 8, 256);
+    if (C <= 32) LAUNCH(32, 1, 2, 3, 32, 256);
+    if (C <= 128) LAUNCH(32, 4, 1, 3, 32, 256);
+    if (C <= 512) LAUNCH(32, 16, 1, 3, 32, 256);
   }
-  const RowWidth w = row_width<VEC>(C);
-  if constexpr (VEC == 4)
-    if (w.pieces == 3) return launch_one<TX, TY, TO, VEC, 0, 3, 1, 2, HASY>(a, w.width, w.threads, st);
-  return launch_one<TX, TY, TO, VEC, 0, 16 / VEC, 1, 2, HASY>(a, w.width, w.threads, st);
+  // long rows: one CTA of 512 threads on an SM leaves half the partial sums that two of 256 do
+  const RowWidth w = row_width<VEC>(C, C * VEC > 2048 ? 512 : 256);
+  if constexpr (VEC == 4) {
+    if (w.pieces == 2) LAUNCH(0, 2, 1, 2, w.width, w.threads);
+    if (w.pieces == 3) LAUNCH(0, 3, 1, 2, w.width, w.threads);
+  }
+  LAUNCH(0, 16 / VEC, 1, VEC == 8 ? 3 : 2, w.width, w.threads);
+#undef LAUNCH
 }
 
 template <class TX, class TY, class TO, bool HASY>
 cudaError_t launch_types(const NormBwdArgs& a, int vec, cudaStream_t st) {
+  const bool dense = a.xs.dense && a.dos.dense && (!HASY || !a.ds || a.dss.dense);
   if constexpr (sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2) {
-    if (vec == 8) return launch_vec<TX, TY, TO, 8, HASY>(a, st);
+    if (vec == 8) return dense ? launch_vec<TX, TY, TO, 8, HASY, true>(a, st) : launch_vec<TX, TY, TO, 8, HASY, false>(a, st);
   }
-  if (vec >= 4) return launch_vec<TX, TY, TO, 4, HASY>(a, st);
-  return launch_vec<TX, TY, TO, 1, HASY>(a, st);
+  if (vec >= 4) return dense ? launch_vec<TX, TY, TO, 4, HASY, true>(a, st) : launch_vec<TX, TY, TO, 4, HASY, false>(a, st);
+  return launch_vec<TX, TY, TO, 1, HASY, false>(a, st);
 }
 
 }  // namespace
 
-int norm_bwd_max_ctas() { return device_sm_count() * kCtasPerSm; }
+int norm_bwd_max_ctas() { return device_sm_count() * kCtasPerSm * kPartials; }
 
 cudaError_t launch_norm_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int dout_dtype, int vec, cudaStream_t st) {
   using H = __half;
