@@ -19,8 +19,10 @@ LIB = PKG / "libtriattn.so"
 RESIDUAL = PKG / "_residual.so"
 RESIDUAL_SOURCE = CSRC / "torch_residual.cpp"
 SOURCES = ["capi.cu", "kernels_f32.cu", "kernels_tc.cu", "noalloc.cu", "peer.cu", "trimul.cu",
-           "residual_capi.cu", "residual_fwd.cu", "residual_bwd.cu", "dropout_add.cu"]
-HEADERS = ["sm100.cuh", "triattn_internal.cuh", "residual.cuh"]
+           "residual_capi.cu", "residual_fwd_norm.cu", "residual_fwd_fused.cu", "residual_fwd_fused16.cu",
+           "residual_fwd_rows.cu", "residual_bwd_norm.cu", "residual_bwd_fused.cu", "residual_bwd_fused16.cu",
+           "dropout_add.cu"]
+HEADERS = ["sm100.cuh", "triattn_internal.cuh", "residual.cuh", "residual_fwd.cuh", "residual_bwd.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,16 +1,20 @@
 // Dropout and dropout + residual add: out = (z ? z : 0) + (keep ? y * scale : 0), residual.cuh's mask.
 //
-// Bound by HBM: z and y read once, out written once; a draw costs about 50 instructions for four
-// positions, which the loads cover.  A thread handles chunks of VEC consecutive elements, U of them in
-// flight.  FLAT: every tensor is dense, so a chunk is VEC consecutive elements of the whole tensor,
-// whatever dim is, and its elements may lie in two rows (or more, for dim < VEC); else a chunk lies in
-// one row.
+// Bound by HBM: z and y read once, out written once; a draw costs about 70 instructions for four positions, which
+// other warps' loads cover as long as enough of them are resident.  A thread handles chunks of VEC consecutive
+// elements, U of them in flight.
 #include "residual.cuh"
 
 namespace triattn {
 namespace {
 
 constexpr int kThreads = 256;
+
+// Where a chunk lies.  kVector: every tensor is dense and every element has a position of its own (or nothing
+// is dropped), so that the tensor is one long vector.  kRows: in one row, found by strides.  kMixed: tensors are
+// dense, but draws are shared and dim is not a multiple of VEC: a chunk is VEC elements of the whole tensor,
+// in two rows or more.
+enum Where { kVector, kRows, kMixed };
 
 // position of the mask of element (row, col)
 __device__ __forceinline__ uint64_t mask_pos(const DropoutAddArgs& a, uint32_t row, uint32_t col) {
@@ -28,8 +32,8 @@ __device__ __forceinline__ void load_some(Pack<T, VEC>& r, const T* p, int n) {
   }
 }
 
-template <class TZ, class TY, class TO, int VEC, int U, bool FLAT, bool HASZ>
-__global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddArgs a, FastDiv per_row,
+template <class TZ, class TY, class TO, int VEC, int U, Where W, bool HASZ>
+__global__ void __launch_bounds__(kThreads, W == kMixed ? 2 : 4) dropout_add_kernel(const DropoutAddArgs a, FastDiv per_row,
                                                                uint64_t elements) {
   const TZ* z = static_cast<const TZ*>(a.z);
   const TY* y = static_cast<const TY*>(a.y);
@@ -37,17 +41,16 @@ __global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddA
   const uint32_t D = (uint32_t)a.dim, drop_max = a.drop.drop_max;
   const float scale = a.drop.scale;
   const Philox rng(a.drop);
+  constexpr bool FLAT = W != kRows;
   const uint64_t chunks = FLAT ? (elements + VEC - 1) / VEC : elements / VEC;
   const uint64_t tiles = (chunks + kThreads * U - 1) / (kThreads * U);
-  const bool row_draw = a.drop.on && !a.drop.per_channel;
-  const bool linear = a.drop.m[2] == (int64_t)D && a.drop.m[1] == (int64_t)D * a.map.n2.d &&
-                      a.drop.m[0] == (int64_t)D * a.map.n2.d * a.map.n1.d;  // every element has its own position
+  const bool row_draw = W != kVector && a.drop.on && !a.drop.per_channel;
   for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const uint64_t first = tile * (kThreads * U);  // chunk
     // first row of the tile and the place in it (elements if FLAT, chunks if not)
     const uint64_t at0 = FLAT ? first * VEC : first;
     uint32_t row_base = 0, rest = 0;
-    if (!FLAT || !linear) {
+    if (W != kVector) {
       row_base = (uint32_t)(at0 / per_row.d);
       rest = (uint32_t)(at0 - (uint64_t)row_base * per_row.d);
     }
@@ -69,7 +72,7 @@ __global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddA
       if constexpr (FLAT) {
         const uint64_t e = (first + q) * VEC;
         if (elements - e < VEC) n[u] = (int)(elements - e);
-        if (!linear) {
+        if (W == kMixed) {
           const uint32_t t = rest + q * VEC, dr = per_row.div(t);
           row[u] = row_base + dr;
           col[u] = t - dr * D;
@@ -84,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddA
         oo[u] = row_offset(a.os, row[u], a.map, D) + col[u];
       }
       if (HASZ && !a.in_place) load_some(zr[u], z + zo, n[u]);
-      if (row_draw && (!FLAT || col[u] + VEC <= D)) kept[u] = rng.word(mask_pos(a, row[u], 0)) > drop_max;
+      if (row_draw && (W == kRows || col[u] + VEC <= D)) kept[u] = rng.word(mask_pos(a, row[u], 0)) > drop_max;
       if (kept[u]) {  // what is dropped whole is not read, and in place not touched
         load_some(yr[u], y + yo, n[u]);
         if (HASZ && a.in_place) load_some(zr[u], z + zo, n[u]);
@@ -102,15 +105,15 @@ __global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddA
         const float v = to_f32(yr[u].v[i]);
         if (k) f[i] = HASZ ? fmaf(v, scale, f[i]) : v * scale;
       };
-      if (!a.drop.on || (row_draw && (!FLAT || col[u] + VEC <= D))) {
+      if (!a.drop.on || (row_draw && (W == kRows || col[u] + VEC <= D))) {
         if (kept[u]) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k) add(true, k);
         }
       } else if (VEC == 1) {
         add(rng.word(mask_pos(a, row[u], col[u])) > drop_max, 0);
-      } else if (!FLAT || linear) {
-        const uint64_t pos = FLAT ? (uint64_t)oo[u] : mask_pos(a, row[u], col[u]);
+      } else if (W != kMixed) {
+        const uint64_t pos = W == kVector ? (uint64_t)oo[u] : mask_pos(a, row[u], col[u]);
 #pragma unroll
         for (int k = 0; k + 3 < VEC; k += 4) {
           const uint4 w = rng.block((pos + k) >> 2);
@@ -156,15 +159,15 @@ __global__ void __launch_bounds__(kThreads) dropout_add_kernel(const DropoutAddA
   }
 }
 
-template <class TZ, class TY, class TO, int VEC, bool FLAT, bool HASZ>
+template <class TZ, class TY, class TO, int VEC, Where W, bool HASZ>
 cudaError_t launch_one(const DropoutAddArgs& a, cudaStream_t st) {
   constexpr int U = VEC == 8 ? 2 : 4;
   const uint64_t elements = (uint64_t)a.map.rows * a.dim;
-  const FastDiv per_row = FastDiv::make(FLAT ? a.dim : a.dim / VEC);
+  const FastDiv per_row = FastDiv::make(W == kRows ? a.dim / VEC : a.dim);
   const uint64_t chunks = (elements + VEC - 1) / VEC, tiles = (chunks + kThreads * U - 1) / (kThreads * U);
-  const uint64_t cap = (uint64_t)device_sm_count() * 32;
-  dropout_add_kernel<TZ, TY, TO, VEC, U, FLAT, HASZ><<<(unsigned)(tiles < cap ? tiles : cap), kThreads, 0, st>>>(
-      a, per_row, elements);
+  // a few tiles a CTA, handed out as SMs come free
+  const uint64_t per = tiles / ((uint64_t)device_sm_count() * 64) + 1, grid = (tiles + per - 1) / per;
+  dropout_add_kernel<TZ, TY, TO, VEC, U, W, HASZ><<<(unsigned)grid, kThreads, 0, st>>>(a, per_row, elements);
   return cudaGetLastError();
 }
 
@@ -172,14 +175,16 @@ template <class TZ, class TY, class TO, bool HASZ>
 cudaError_t launch_types(const DropoutAddArgs& a, int vec, cudaStream_t st) {
   constexpr int FULL = sizeof(TZ) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2 ? 8 : 4;
   const auto aligned = [](const void* p, size_t b) { return reinterpret_cast<uintptr_t>(p) % b == 0; };
-  // A dense tensor of independent draws is one long vector; with shared draws a row's chunks need their row.
   const bool flat = (!a.z || a.zs.dense) && a.ys.dense && a.os.dense && aligned(a.z, FULL * sizeof(TZ)) &&
                     aligned(a.y, FULL * sizeof(TY)) && aligned(a.out, FULL * sizeof(TO));
-  const bool shared = a.drop.on && a.drop.m[0] * a.drop.m[1] * a.drop.m[2] * a.drop.per_channel == 0;
-  if (flat && !shared) return launch_one<TZ, TY, TO, FULL, true, HASZ>(a, st);
-  if (vec >= FULL) return launch_one<TZ, TY, TO, FULL, false, HASZ>(a, st);
-  if (flat) return launch_one<TZ, TY, TO, FULL, true, HASZ>(a, st);
-  return launch_one<TZ, TY, TO, 1, false, HASZ>(a, st);
+  const int64_t m2 = a.dim, m1 = m2 * a.map.n2.d, m0 = m1 * a.map.n1.d;
+  const bool own = !a.drop.on || (a.drop.per_channel && (a.map.n2.d == 1 || a.drop.m[2] == m2) &&
+                                  (a.map.n1.d == 1 || a.drop.m[1] == m1) &&
+                                  (a.map.rows == a.map.n1.d * a.map.n2.d || a.drop.m[0] == m0));
+  if (flat && own) return launch_one<TZ, TY, TO, FULL, kVector, HASZ>(a, st);
+  if (vec >= FULL) return launch_one<TZ, TY, TO, FULL, kRows, HASZ>(a, st);
+  if (flat) return launch_one<TZ, TY, TO, FULL, kMixed, HASZ>(a, st);
+  return launch_one<TZ, TY, TO, 1, kRows, HASZ>(a, st);
 }
 
 }  // namespace

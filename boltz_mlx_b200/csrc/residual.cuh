@@ -43,14 +43,52 @@ struct Strides3 {
 struct RowIndex {
   uint32_t i0, i1, i2;
 };
+// The order in which a call's rows are worked on: row after row, or, where some tensor is transposed against
+// the others, in squares of 8 x 8 of the last two axes, i1 fastest, so that both kinds of tensor are touched in
+// runs of 8 rows that are neighbours in memory (the squares at the edge are filled up with places that hold
+// no row).
 struct RowMap {
-  uint32_t rows;
+  uint32_t rows;    // that there are
+  uint32_t places;  // in the order of work
   FastDiv n1, n2;
-  __device__ __forceinline__ RowIndex at(uint32_t row) const {
-    const uint32_t q = n2.div(row), i0 = n1.div(q);
-    return RowIndex{i0, q - i0 * n1.d, row - q * n2.d};
+  bool tiled;
+  FastDiv t1, t2;  // squares along i1 and i2
+  static RowMap make(const int64_t* n, int64_t rows, bool tiled) {
+    const auto size = [](int64_t v) { return (uint32_t)(v > 0 ? v : 1); };
+    RowMap m{};
+    m.rows = m.places = (uint32_t)rows;
+    m.n1 = FastDiv::make(size(n[1]));
+    m.n2 = FastDiv::make(size(n[2]));
+    const int64_t a = (n[1] + 7) / 8, b = (n[2] + 7) / 8;
+    m.tiled = tiled && n[1] > 1 && n[2] > 1 && n[0] * a * b * 64 < 0x7fffffffLL - (1 << 20);
+    m.t1 = FastDiv::make(size(a));
+    m.t2 = FastDiv::make(size(b));
+    if (m.tiled) m.places = (uint32_t)(n[0] * a * b * 64);
+    return m;
+  }
+  __device__ __forceinline__ RowIndex at(uint32_t place) const {
+    if (tiled) {
+      const uint32_t q = place >> 6, i = t2.div(q), i0 = t1.div(i);
+      return RowIndex{i0, (i - i0 * t1.d) * 8 + (place & 7), (q - i * t2.d) * 8 + (place >> 3 & 7)};
+    }
+    const uint32_t q = n2.div(place), i0 = n1.div(q);
+    return RowIndex{i0, q - i0 * n1.d, place - q * n2.d};
   }
 };
+// A place of that order and its row.
+template <bool DENSE>
+struct Spot {
+  uint32_t row;  // DENSE: the place
+  RowIndex i;    // not DENSE
+  bool live;     // there is a row
+  __device__ __forceinline__ RowIndex index(const RowMap& map) const {
+    if constexpr (DENSE)
+      return map.at(row);
+    else
+      return i;
+  }
+};
+
 __device__ __forceinline__ int64_t row_offset(const Strides3& s, uint32_t row, const RowMap& map, int dim) {
   if (s.dense) return (int64_t)row * dim;
   const RowIndex i = map.at(row);
@@ -277,7 +315,7 @@ __device__ __forceinline__ void copy_wait() {
 // not, its place in shared memory holds zeros.
 // VEC = 1, for rows that start anywhere (an odd dim, an odd stride or address): the row's lanes copy the
 // 16-byte blocks that hold it, so what a lane reads was copied by its neighbours, and a barrier of the
-// row's lanes (sync) stands before and after the reading.
+// row's lanes (sync) stands before and after the reading.  All pieces but the last four are there.
 constexpr int RES_MAX_WARPS = 16;  // of a CTA
 constexpr int RES_MAX_GROUPS = 8;  // of several warps, in a CTA
 constexpr int RES_MAX_SUMS = 4;    // of one call
@@ -294,7 +332,7 @@ struct Lanes {
     last = col(NCH - 1) < dim;
   }
   __device__ __forceinline__ bool act(int c) const {
-    return VEC > 1 ? (c < NCH - 1 || last) : col(c) < dim;
+    return VEC > 1 ? (c < NCH - 1 || last) : (c < NCH - 4 || col(c) < dim);
   }
   __device__ __forceinline__ int col(int c) const { return (lane + c * width) * VEC; }
   __device__ __forceinline__ void barrier() const {  // of the row's lanes
@@ -349,6 +387,38 @@ struct Lanes {
   }
 };
 
+// The R places from `place` on.  Where rows are found by their index, lane r of a group finds that of place r
+// and hands it round: one search a lane instead of R.
+template <bool DENSE, int R, int VEC, int LPR, int NCH>
+__device__ __forceinline__ void spots(const Lanes<VEC, LPR, NCH>& l, const RowMap& map, uint32_t place, Spot<DENSE> (&s)[R]) {
+  if constexpr (DENSE) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r].row = place + r;
+      s[r].live = place + r < map.places;
+    }
+  } else {
+    static_assert((R & (R - 1)) == 0 && (LPR || R == 1), "");
+    const uint32_t mine = place + (l.lane & (R - 1));
+    const RowIndex i = map.at(mine);
+    const bool live = mine < map.places && i.i1 < map.n1.d && i.i2 < map.n2.d;
+    const uint32_t row = live ? (i.i0 * map.n1.d + i.i1) * map.n2.d + i.i2 : ~0u;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if constexpr (R > 1) {
+        s[r].row = __shfl_sync(0xffffffffu, row, r, LPR);
+        s[r].i.i0 = __shfl_sync(0xffffffffu, i.i0, r, LPR);
+        s[r].i.i1 = __shfl_sync(0xffffffffu, i.i1, r, LPR);
+        s[r].i.i2 = __shfl_sync(0xffffffffu, i.i2, r, LPR);
+      } else {
+        s[r].row = row;
+        s[r].i = i;
+      }
+      s[r].live = s[r].row != ~0u;
+    }
+  }
+}
+
 // Rows of several warps: C pieces (of VEC channels) on `width` lanes, 16 channels a lane at most (registers); the
 // number of pieces a lane that leaves the fewest lanes idle, all but the last full.
 struct RowWidth {
@@ -358,14 +428,13 @@ template <int VEC>
 RowWidth row_width(int C, int threads) {  // a CTA of about so many threads
   RowWidth best{16 / VEC, 512, 512};
   int cost = 1 << 30;
-  for (int n = 16 / VEC; n >= 2; --n) {
+  for (int n = 16 / VEC; n >= 2; n -= VEC == 1 ? 4 : 1) {
     const int width = ((C + n - 1) / n + 31) / 32 * 32;
-    if (width > 512 || (VEC > 1 && (n - 1) * width > C)) continue;
+    if (width > 512 || (VEC > 1 ? (n - 1) * width > C : (n < 12 || (n - 4) * width >= C))) continue;
     if (width * n < cost) {
       cost = width * n;
       best = RowWidth{n, width, width < threads ? threads / width * width : width};
     }
-    if (VEC != 4) break;
   }
   return best;
 }
@@ -392,13 +461,11 @@ struct RowsOf {
       s2 = s.s[2] * (int)sizeof(T);
     }
   }
-  __device__ __forceinline__ T* at(uint32_t row, const RowMap& map) const {
-    if constexpr (DENSE) {
-      return reinterpret_cast<T*>(base + (uint64_t)row * pitch);
-    } else {
-      const RowIndex i = map.at(row);
-      return reinterpret_cast<T*>(base + s0 * i.i0 + s1 * i.i1 + s2 * i.i2);
-    }
+  __device__ __forceinline__ T* at(const Spot<DENSE>& p) const {
+    if constexpr (DENSE)
+      return reinterpret_cast<T*>(base + (uint64_t)p.row * pitch);
+    else
+      return reinterpret_cast<T*>(base + s0 * p.i.i0 + s1 * p.i.i1 + s2 * p.i.i2);
   }
 };
 
@@ -410,12 +477,11 @@ struct RowIn {
   static constexpr int B = VEC * sizeof(T);
   static_assert(VEC == 1 || B == 8 || B == 16, "");
   const L& l;
-  const RowMap& map;
   RowsOf<T, DENSE> rows;
   char* ring;  // VEC > 1: at the lane's first piece
   uint32_t ring32;
-  __device__ __forceinline__ RowIn(const L& l_, const RowMap& m, const void* p, const Strides3& s, char* r)
-      : l(l_), map(m), rows(p, s, l_.dim, VEC > 1 ? l_.lane * VEC : 0) {
+  __device__ __forceinline__ RowIn(const L& l_, const void* p, const Strides3& s, char* r)
+      : l(l_), rows(p, s, l_.dim, VEC > 1 ? l_.lane * VEC : 0) {
     ring = r + (VEC > 1 ? l.lane * B : 0);
     ring32 = smem_u32(ring);
   }
@@ -430,8 +496,8 @@ struct RowIn {
       }
     }
   }
-  __device__ __forceinline__ void issue(int off, uint32_t row) const {
-    const T* p = rows.at(row, map);
+  __device__ __forceinline__ void issue(int off, const Spot<DENSE>& spot) const {
+    const T* p = rows.at(spot);
     if constexpr (VEC > 1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c)
@@ -445,14 +511,17 @@ struct RowIn {
         copy_async_part(dst, reinterpret_cast<const void*>(at), end - at < 16 ? (int)(end - at) : 16);
     }
   }
-  // a row that is not there: zeros (VEC > 1; elsewhere read() takes care of it)
+  // a row that is not there: zeros
   __device__ __forceinline__ void issue_none(int off) const {
     if constexpr (VEC > 1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) copy_zero<B>(ring32 + off + c * step(), rows.base);
+    } else {
+      for (int i = l.lane * 16; i < row_slot<T, VEC, NCH>(l.width, l.dim); i += l.width * 16)
+        copy_zero<16>(ring32 + off + i, rows.base);
     }
   }
-  __device__ __forceinline__ void read(int off, uint32_t row, bool live, Pair (&x)[L::PAIRS]) const {
+  __device__ __forceinline__ void read(int off, const Spot<DENSE>& spot, Pair (&x)[L::PAIRS]) const {
     if constexpr (VEC > 1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
@@ -461,10 +530,10 @@ struct RowIn {
         for (int j = 0; j < VEC / 2; ++j) x[c * VEC / 2 + j] = to_pair(p.v + 2 * j);
       }
     } else {
-      const T* p = reinterpret_cast<const T*>(ring + off + (reinterpret_cast<uintptr_t>(rows.at(row, map)) & 15));
+      const T* p = reinterpret_cast<const T*>(ring + off + (reinterpret_cast<uintptr_t>(rows.at(spot)) & 15));
       float v[2 * L::PAIRS];
 #pragma unroll
-      for (int c = 0; c < 2 * L::PAIRS; ++c) v[c] = c < NCH && live && l.act(c) ? to_f32(p[l.col(c)]) : 0.0f;
+      for (int c = 0; c < 2 * L::PAIRS; ++c) v[c] = c < NCH && l.act(c) ? to_f32(p[l.col(c)]) : 0.0f;
 #pragma unroll
       for (int j = 0; j < L::PAIRS; ++j) x[j] = pair(v[2 * j], v[2 * j + 1]);
     }
@@ -475,12 +544,10 @@ template <class T, int VEC, int LPR, int NCH, bool DENSE>
 struct RowOut {
   using L = Lanes<VEC, LPR, NCH>;
   const L& l;
-  const RowMap& map;
   RowsOf<T, DENSE> rows;
-  __device__ __forceinline__ RowOut(const L& l_, const RowMap& m, const void* p, const Strides3& s)
-      : l(l_), map(m), rows(p, s, l_.dim, l_.lane * VEC) {}
-  __device__ __forceinline__ T* at(uint32_t row) const { return rows.at(row, map); }
-  // piece c of a row's values, if the lane has it; p = at(row)
+  __device__ __forceinline__ RowOut(const L& l_, const void* p, const Strides3& s) : l(l_), rows(p, s, l_.dim, l_.lane * VEC) {}
+  __device__ __forceinline__ T* at(const Spot<DENSE>& spot) const { return rows.at(spot); }
+  // piece c of a row's values, if the lane has it; p = at(its spot)
   __device__ __forceinline__ void piece(T* p, int c, const Pair (&x)[L::PAIRS]) const {
     if (!l.act(c)) return;
     if constexpr (VEC > 1) {
@@ -493,8 +560,8 @@ struct RowOut {
       p[c * l.width] = from_f32<T>(c & 1 ? h.y : h.x);
     }
   }
-  __device__ __forceinline__ void row(uint32_t row, const Pair (&x)[L::PAIRS]) const {
-    T* p = at(row);
+  __device__ __forceinline__ void row(const Spot<DENSE>& spot, const Pair (&x)[L::PAIRS]) const {
+    T* p = at(spot);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) piece(p, c, x);
   }
@@ -558,8 +625,13 @@ __device__ __forceinline__ void centre(const Lanes<VEC, LPR, NCH>& l, Pair m, Pa
   } else {
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-      const float2 a = halves(x[j]), d = halves(x[j] + m);
-      x[j] = pair(l.act(2 * j) ? d.x : a.x, 2 * j + 1 < NCH && l.act(2 * j + 1) ? d.y : a.y);
+      const Pair d = x[j] + m;
+      if (2 * j + 1 < NCH - 4) {
+        x[j] = d;
+      } else {
+        const float2 h = halves(d);
+        x[j] = pair(l.act(2 * j) ? h.x : 0.0f, 2 * j + 1 < NCH && l.act(2 * j + 1) ? h.y : 0.0f);
+      }
       t = fma2(x[j], x[j], t);
     }
   }
@@ -607,7 +679,8 @@ __device__ __forceinline__ void each_kept(const Lanes<VEC, LPR, NCH>& l, const P
 int device_sm_count();
 
 // ---- arguments ------------------------------------------------------------------------------------
-// forward: out = LN(x), x = z, or (with y) x = s = z + dropout(y) rounded to z's type and stored in sum
+// forward: out = LN(x), x = z, or (with y) x = s = z + dropout(y) rounded to sum's type (z's) and stored in sum;
+// the sum alone, with or without z, for triattn_dropout_add
 struct NormFwdArgs {
   const void *z, *y;
   void *sum, *out;
@@ -618,6 +691,7 @@ struct NormFwdArgs {
   int param_dtype;
   float eps;
   float *mean, *rstd;  // [rows] or nullptr
+  int in_place;        // sum is z
   Dropout drop;
 };
 // backward: dx = ds + LN'(dout), dy = dropout(dx), partial column sums of dout * xhat and dout
@@ -689,12 +763,17 @@ struct KernelInfo {
   }
 };
 
-// what every tensor of a call allows: elements moved at a time (8, 4 or 1)
-cudaError_t launch_norm_fwd(const NormFwdArgs& a, int z_dtype, int y_dtype, int out_dtype, int vec, cudaStream_t st);
-cudaError_t launch_norm_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int dout_dtype, int vec, cudaStream_t st);
+// vec: what every tensor of a call allows, elements moved at a time (8, 4 or 1)
+cudaError_t launch_norm_fwd(const NormFwdArgs& a, int z_dtype, int out_dtype, int vec, cudaStream_t st);
+cudaError_t launch_fused_fwd(const NormFwdArgs& a, int z_dtype, int y_dtype, int out_dtype, int vec, cudaStream_t st);
+cudaError_t launch_fused16_fwd(const NormFwdArgs& a, int z_dtype, int y_dtype, int out_dtype, int vec, cudaStream_t st);
+cudaError_t launch_norm_bwd(const NormBwdArgs& a, int x_dtype, int dout_dtype, int vec, cudaStream_t st);
+cudaError_t launch_fused_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int dout_dtype, int vec, cudaStream_t st);
+cudaError_t launch_fused16_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int dout_dtype, int vec, cudaStream_t st);
 cudaError_t launch_dropout_add(const DropoutAddArgs& a, int z_dtype, int y_dtype, int out_dtype, int vec,
                                cudaStream_t st);
-// CTAs of launch_norm_bwd at most (rows of its partial sums)
-int norm_bwd_max_ctas();
+// triattn_dropout_add over dense rows of which each is dropped or kept whole; vec 4 or 8, dim up to 64 vec (128 for 4)
+cudaError_t launch_dropout_rows(const NormFwdArgs& a, int y_dtype, int out_dtype, int vec, cudaStream_t st);
+int norm_bwd_max_ctas();  // of a launch: rows of its partial sums
 
 }  // namespace triattn

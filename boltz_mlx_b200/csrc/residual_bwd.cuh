@@ -9,6 +9,7 @@
 // registers until the CTA has seen its last row; they are then joined in shared memory, written as one
 // partial row per CTA and summed by a second small kernel in the order of the CTAs: no atomics, the same
 // bits on every run.
+#pragma once
 #include <cooperative_groups.h>
 
 #include "residual.cuh"
@@ -16,11 +17,11 @@
 namespace triattn {
 namespace {
 
-constexpr int kCtasPerSm = 4;   // resident at most
+constexpr int kCtasPerSm = 4;  // resident at most
 constexpr int kPartials = 5;   // CTAs of a launch at most, times those
 
 template <class TX, class TO, int VEC, int NCH, int R, bool HASY>
-constexpr int stage_bytes(int width, int dim) {
+constexpr int bwd_stage_bytes(int width, int dim) {
   return R * ((HASY ? 2 : 1) * row_slot<TX, VEC, NCH>(width, dim) + row_slot<TO, VEC, NCH>(width, dim));
 }
 
@@ -45,12 +46,12 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
   const bool row_draw = has_dy && a.drop.on && !a.drop.per_channel, draw = has_dy && a.drop.on && a.drop.per_channel;
 
   const int slot_x = row_slot<TX, VEC, NCH>(l.width, D), slot_o = row_slot<TO, VEC, NCH>(l.width, D);
-  const int stage = stage_bytes<TX, TO, VEC, NCH, R, HASY>(l.width, D);
+  const int stage = bwd_stage_bytes<TX, TO, VEC, NCH, R, HASY>(l.width, D);
   char* ring = smem + l.group * S * stage;
-  const RowIn<TX, VEC, LPR, NCH, DENSE> x(l, a.map, a.x, a.xs, ring), ds(l, a.map, a.ds, a.dss, ring + R * (slot_x + slot_o));
-  const RowIn<TO, VEC, LPR, NCH, DENSE> dout(l, a.map, a.dout, a.dos, ring + R * slot_x);
-  const RowOut<TX, VEC, LPR, NCH, true> dx(l, a.map, a.dx, a.xs);
-  const RowOut<TY, VEC, LPR, NCH, true> dy(l, a.map, a.dy, a.xs);
+  const RowIn<TX, VEC, LPR, NCH, DENSE> x(l, a.x, a.xs, ring), ds(l, a.ds, a.dss, ring + R * (slot_x + slot_o));
+  const RowIn<TO, VEC, LPR, NCH, DENSE> dout(l, a.dout, a.dos, ring + R * slot_x);
+  const RowOut<TX, VEC, LPR, NCH, true> dx(l, a.dx, a.xs);
+  const RowOut<TY, VEC, LPR, NCH, true> dy(l, a.dy, a.xs);
   for (int k = 0; k < S; ++k) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -60,29 +61,32 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     }
   }
 
-  const uint32_t rows = a.map.rows, step = l.groups * R;
+  const RowMap& map = a.map;
+  const uint32_t step = l.groups * R;
   const auto issue = [&](uint32_t base, int s) {
+    Spot<DENSE> spot[R];
+    spots(l, map, base + l.group * R, spot);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t row = base + l.group * R + r;
-      if (row >= rows) {  // adds nothing to the column sums
+      if (!spot[r].live) {  // adds nothing to the column sums
         x.issue_none(s * stage + r * slot_x);
         dout.issue_none(s * stage + r * slot_o);
         continue;
       }
-      x.issue(s * stage + r * slot_x, row);
-      dout.issue(s * stage + r * slot_o, row);
+      x.issue(s * stage + r * slot_x, spot[r]);
+      dout.issue(s * stage + r * slot_o, spot[r]);
       if constexpr (HASY)
-        if (has_ds) ds.issue(s * stage + r * slot_x, row);
+        if (has_ds) ds.issue(s * stage + r * slot_x, spot[r]);
     }
   };
   float mean_next[R], rstd_next[R];  // of the next batch
+  Spot<DENSE> next[R];
   const auto statistics = [&](uint32_t base) {
+    spots(l, map, base + l.group * R, next);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t row = base + l.group * R + r;
-      mean_next[r] = row < rows ? a.mean[row] : 0.0f;
-      rstd_next[r] = row < rows ? a.rstd[row] : 0.0f;
+      mean_next[r] = next[r].live ? a.mean[next[r].row] : 0.0f;
+      rstd_next[r] = next[r].live ? a.rstd[next[r].row] : 0.0f;
     }
   };
 
@@ -102,24 +106,23 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     if (ahead < end) issue(ahead, s == 0 ? S - 1 : s - 1);
     copy_commit();
     float mean[R], rstd[R];
+    Spot<DENSE> spot[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      spot[r] = next[r];
       mean[r] = mean_next[r];
       rstd[r] = rstd_next[r];
     }
     statistics(base + step);
     copy_wait<S - 1>();
     l.sync();
-    const uint32_t row0 = base + l.group * R;
     // v[2 r] = sum g, v[2 r + 1] = sum g xh
     Pair xh[R][P], g[R][P];
     float v[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t row = row0 + r;
-      const bool live = row < rows;
-      x.read(s * stage + r * slot_x, row, live, xh[r]);
-      dout.read(s * stage + r * slot_o, row, live, g[r]);
+      x.read(s * stage + r * slot_x, spot[r], xh[r]);
+      dout.read(s * stage + r * slot_o, spot[r], g[r]);
       const Pair q = both(rstd[r]), mq = both(-mean[r] * rstd[r]);
       Pair s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
@@ -138,23 +141,25 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     uint32_t whole = ~0u;  // bit r: row r is not dropped whole
     if constexpr (HASY) {
       if (row_draw) {
+        const int mine = LPR ? l.lane & (R - 1) : 0;
+        RowIndex i = spot[0].index(map);
+        if constexpr (DENSE)
+          i = map.at(spot[0].row + mine);
+        else
+#pragma unroll
+          for (int r = 1; r < R; ++r)
+            if (r == mine) i = spot[r].i;
+        const bool k = rng.word(mask_base(a.drop, i)) > a.drop.drop_max;
         whole = 0;
-        if constexpr (LPR && R > 1) {
-          const uint32_t row = row0 + (l.lane & (R - 1));
-          const bool k = row < rows && rng.word(mask_base(a.drop, a.map.at(row))) > a.drop.drop_max;
 #pragma unroll
-          for (int r = 0; r < R; ++r) whole |= __shfl_sync(0xffffffffu, (uint32_t)k, r, LPR) << r;
-        } else {
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (row0 + r < rows && rng.word(mask_base(a.drop, a.map.at(row0 + r))) > a.drop.drop_max) whole |= 1u << r;
-        }
+        for (int r = 0; r < R; ++r)
+          whole |= (R > 1 ? __shfl_sync(0xffffffffu, (uint32_t)k, r, LPR ? LPR : 32) : (uint32_t)k) << r;
       }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t row = row0 + r;
-      const bool live = row < rows;
+      const bool live = spot[r].live;
+      const Spot<true> to{spot[r].row, {}, live};
       const float t = -inv_d * rstd[r];
       const Pair c1 = both(v[2 * r] * t), c2 = both(v[2 * r + 1] * t), q = both(rstd[r]);
 #pragma unroll
@@ -162,16 +167,16 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
       if constexpr (HASY) {
         if (has_ds) {
           Pair sv[P];
-          ds.read(s * stage + r * slot_x, row, live, sv);
+          ds.read(s * stage + r * slot_x, spot[r], sv);
 #pragma unroll
           for (int j = 0; j < P; ++j) g[r][j] = g[r][j] + sv[j];
         }
       }
-      if (a.dx && live) dx.row(row, g[r]);
+      if (a.dx && live) dx.row(to, g[r]);
       if constexpr (HASY) {
         if (has_dy) {
           if (draw) {
-            each_kept(l, rng, mask_base(a.drop, a.map.at(live ? row : rows - 1)), a.drop.drop_max, [&](bool k, int i) {
+            each_kept(l, rng, mask_base(a.drop, spot[r].index(map)), a.drop.drop_max, [&](bool k, int i) {
               const float2 gi = halves(g[r][i / 2]);
               const float f = k ? (i & 1 ? gi.y : gi.x) * a.drop.scale : 0.0f;
               g[r][i / 2] = i & 1 ? pair(gi.x, f) : pair(f, gi.y);
@@ -181,7 +186,7 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
 #pragma unroll
             for (int j = 0; j < P; ++j) g[r][j] = whole >> r & 1 ? g[r][j] * scale : both(0.0f);
           }
-          if (live) dy.row(row, g[r]);
+          if (live) dy.row(to, g[r]);
         }
       }
     }
@@ -225,9 +230,9 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
 
 // Column sums of the CTAs' partial rows: a cluster of kJoin CTAs for 32 columns, each of its warps with every
 // 16 * kJoin-th row; the cluster's first CTA adds up what the others hold in their shared memory.  One CTA
-// alone needs 15 us for the 2000 partial rows of a long launch, the cluster 3.
-constexpr int kJoin = 8;
-template <class TP>
+// alone needs 15 us for the 2000 partial rows of a long launch, a cluster of eight 3; for the few partial rows
+// of a short launch, or the many columns of long rows, one is enough.
+template <class TP, int kJoin>
 __global__ void __cluster_dims__(kJoin, 1, 1) __launch_bounds__(512)
     norm_bwd_join_kernel(const float* __restrict__ partial, int ctas, int dim, TP* __restrict__ dweight,
                          TP* __restrict__ dbias) {
@@ -264,6 +269,17 @@ __global__ void __cluster_dims__(kJoin, 1, 1) __launch_bounds__(512)
   cluster.sync();  // no CTA leaves while its sums are read
 }
 
+template <class TP>
+cudaError_t launch_join(const NormBwdArgs& a, int ctas, cudaStream_t st) {
+  const int blocks = (2 * a.dim + 31) / 32;
+  TP *dw = static_cast<TP*>(a.dweight), *db = static_cast<TP*>(a.dbias);
+  if (ctas > 320 && blocks <= 64)
+    norm_bwd_join_kernel<TP, 8><<<blocks * 8, 512, 0, st>>>(a.partial, ctas, a.dim, dw, db);
+  else
+    norm_bwd_join_kernel<TP, 1><<<blocks, 512, 0, st>>>(a.partial, ctas, a.dim, dw, db);
+  return cudaGetLastError();
+}
+
 // Three quarters of the batches go to the CTAs that are resident from the start, in equal shares; the rest in
 // shares an eighth as large, to whichever SM comes free: equal shares alone leave the SMs that the memory
 // system serves last working alone at the end.  Every CTA costs a partial row of 16 bytes a channel (written
@@ -283,39 +299,31 @@ Split share(uint32_t batches, uint32_t resident, uint32_t per) {
 }
 
 template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY, bool DENSE>
-cudaError_t launch_one(const NormBwdArgs& a, int width, int threads, cudaStream_t st) {
+cudaError_t bwd_one(const NormBwdArgs& a, int width, int threads, cudaStream_t st) {
   static KernelInfo info;
   const int groups = threads / width, sets = LPR ? threads / 32 : groups;
-  size_t smem = (size_t)groups * S * stage_bytes<TX, TO, VEC, NCH, R, HASY>(width, a.dim);
+  size_t smem = (size_t)groups * S * bwd_stage_bytes<TX, TO, VEC, NCH, R, HASY>(width, a.dim);
   if (const size_t sums = (size_t)sets * 2 * a.dim * 4; sets > 1 && smem < sums) smem = sums;
   int fit = 0;
   if (cudaError_t e = info.fit(norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE>, threads, smem, &fit);
       e != cudaSuccess)
     return e;
   if (fit > kCtasPerSm) fit = kCtasPerSm;
-  const uint32_t per = groups * R, batches = ((uint32_t)a.map.rows + per - 1) / per;
+  const uint32_t per = groups * R, batches = (a.map.places + per - 1) / per;
   const Split split = share(batches, (uint32_t)(device_sm_count() * fit), per);
   const uint32_t grid = split.big + (split.few ? (batches - split.big * split.many + split.few - 1) / split.few : 0);
   norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE><<<grid, threads, smem, st>>>(a, width, split);
   if (cudaError_t e = cudaGetLastError(); e != cudaSuccess || !a.partial) return e;
-  const int blocks = (2 * a.dim + 31) / 32 * kJoin;
-  if (a.param_dtype == DT_F32)
-    norm_bwd_join_kernel<<<blocks, 512, 0, st>>>(a.partial, (int)grid, a.dim, static_cast<float*>(a.dweight),
-                                                static_cast<float*>(a.dbias));
-  else if (a.param_dtype == DT_F16)
-    norm_bwd_join_kernel<<<blocks, 512, 0, st>>>(a.partial, (int)grid, a.dim, static_cast<__half*>(a.dweight),
-                                                static_cast<__half*>(a.dbias));
-  else
-    norm_bwd_join_kernel<<<blocks, 512, 0, st>>>(a.partial, (int)grid, a.dim, static_cast<__nv_bfloat16*>(a.dweight),
-                                                static_cast<__nv_bfloat16*>(a.dbias));
-  return cudaGetLastError();
+  if (a.param_dtype == DT_F32) return launch_join<float>(a, (int)grid, st);
+  if (a.param_dtype == DT_F16) return launch_join<__half>(a, (int)grid, st);
+  return launch_join<__nv_bfloat16>(a, (int)grid, st);
 }
 
 template <class TX, class TY, class TO, int VEC, bool HASY, bool DENSE>
-cudaError_t launch_vec(const NormBwdArgs& a, cudaStream_t st) {
+cudaError_t bwd_vec(const NormBwdArgs& a, cudaStream_t st) {
   const int C = (a.dim + VEC - 1) / VEC;
 #define LAUNCH(LPR, NCH, R, S, WIDTH, THREADS) \
-  return launch_one<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE>(a, WIDTH, THREADS, st)
+  return bwd_one<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE>(a, WIDTH, THREADS, st)
   if constexpr (VEC > 1) {
     if (C <= 8) LAUNCH(8, 1, 4, 2, 8, 256);
     if (C <= 16) LAUNCH(16, 1, 4, 2, 16, 256);
@@ -326,9 +334,10 @@ cudaError_t launch_vec(const NormBwdArgs& a, cudaStream_t st) {
       if (C <= 128) LAUNCH(32, 4, 1, 3, 32, 256);
     }
   } else {
-    if (C <= 8) LAUNCH(8, 1, 2, 3, 8, 256);
     if (C <= 32) LAUNCH(32, 1, 2, 3, 32, 256);
-    if (C <= 128) LAUNCH(32, 4, 1, 3, 32, 256);
+    if (C <= 128) LAUNCH(32, 4, 2, 2, 32, 256);
+    if (C <= 256) LAUNCH(32, 8, 1, 3, 32, 256);
+    if (C <= 384) LAUNCH(32, 12, 1, 3, 32, 256);
     if (C <= 512) LAUNCH(32, 16, 1, 3, 32, 256);
   }
   // long rows: one CTA of 512 threads on an SM leaves half the partial sums that two of 256 do
@@ -337,45 +346,19 @@ cudaError_t launch_vec(const NormBwdArgs& a, cudaStream_t st) {
     if (w.pieces == 2) LAUNCH(0, 2, 1, 2, w.width, w.threads);
     if (w.pieces == 3) LAUNCH(0, 3, 1, 2, w.width, w.threads);
   }
+  if constexpr (VEC == 1)
+    if (w.pieces == 12) LAUNCH(0, 12, 1, 2, w.width, w.threads);
   LAUNCH(0, 16 / VEC, 1, VEC == 8 ? 3 : 2, w.width, w.threads);
 #undef LAUNCH
 }
 
 template <class TX, class TY, class TO, bool HASY>
-cudaError_t launch_types(const NormBwdArgs& a, int vec, cudaStream_t st) {
+cudaError_t bwd_types(const NormBwdArgs& a, int vec, cudaStream_t st) {
   const bool dense = a.xs.dense && a.dos.dense && (!HASY || !a.ds || a.dss.dense);
-  if constexpr (sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2) {
-    if (vec == 8) return dense ? launch_vec<TX, TY, TO, 8, HASY, true>(a, st) : launch_vec<TX, TY, TO, 8, HASY, false>(a, st);
-  }
-  if (vec >= 4) return dense ? launch_vec<TX, TY, TO, 4, HASY, true>(a, st) : launch_vec<TX, TY, TO, 4, HASY, false>(a, st);
-  return launch_vec<TX, TY, TO, 1, HASY, false>(a, st);
+  constexpr int FULL = sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2 ? 8 : 4;
+  if (vec >= FULL) return dense ? bwd_vec<TX, TY, TO, FULL, HASY, true>(a, st) : bwd_vec<TX, TY, TO, FULL, HASY, false>(a, st);
+  return dense ? bwd_vec<TX, TY, TO, 1, HASY, true>(a, st) : bwd_vec<TX, TY, TO, 1, HASY, false>(a, st);
 }
 
 }  // namespace
-
-int norm_bwd_max_ctas() { return device_sm_count() * kCtasPerSm * kPartials; }
-
-cudaError_t launch_norm_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int dout_dtype, int vec, cudaStream_t st) {
-  using H = __half;
-  using B = __nv_bfloat16;
-  if (!a.dy && !a.ds) {
-    if (x_dtype == DT_F32 && dout_dtype == DT_F32) return launch_types<float, float, float, false>(a, vec, st);
-    if (x_dtype == DT_F32 && dout_dtype == DT_F16) return launch_types<float, float, H, false>(a, vec, st);
-    if (x_dtype == DT_F32 && dout_dtype == DT_BF16) return launch_types<float, float, B, false>(a, vec, st);
-    if (x_dtype == DT_F16 && dout_dtype == DT_F16) return launch_types<H, H, H, false>(a, vec, st);
-    if (x_dtype == DT_BF16 && dout_dtype == DT_BF16) return launch_types<B, B, B, false>(a, vec, st);
-    return cudaErrorInvalidValue;
-  }
-  if (x_dtype == DT_F32 && y_dtype == DT_F32) {
-    if (dout_dtype == DT_F32) return launch_types<float, float, float, true>(a, vec, st);
-    if (dout_dtype == DT_F16) return launch_types<float, float, H, true>(a, vec, st);
-    if (dout_dtype == DT_BF16) return launch_types<float, float, B, true>(a, vec, st);
-  }
-  if (x_dtype == DT_F32 && y_dtype == DT_F16 && dout_dtype == DT_F16) return launch_types<float, H, H, true>(a, vec, st);
-  if (x_dtype == DT_F32 && y_dtype == DT_BF16 && dout_dtype == DT_BF16) return launch_types<float, B, B, true>(a, vec, st);
-  if (x_dtype == DT_F16 && y_dtype == DT_F16 && dout_dtype == DT_F16) return launch_types<H, H, H, true>(a, vec, st);
-  if (x_dtype == DT_BF16 && y_dtype == DT_BF16 && dout_dtype == DT_BF16) return launch_types<B, B, B, true>(a, vec, st);
-  return cudaErrorInvalidValue;
-}
-
 }  // namespace triattn
