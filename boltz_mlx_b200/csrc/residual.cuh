@@ -43,52 +43,18 @@ struct Strides3 {
 struct RowIndex {
   uint32_t i0, i1, i2;
 };
-// The order in which a call's rows are worked on: row after row, or, where some tensor is transposed against
-// the others, in squares of 8 x 8 of the last two axes, i1 fastest, so that both kinds of tensor are touched in
-// runs of 8 rows that are neighbours in memory (the squares at the edge are filled up with places that hold
-// no row).
 struct RowMap {
-  uint32_t rows;    // that there are
-  uint32_t places;  // in the order of work
+  uint32_t rows;
   FastDiv n1, n2;
-  bool tiled;
-  FastDiv t1, t2;  // squares along i1 and i2
-  static RowMap make(const int64_t* n, int64_t rows, bool tiled) {
+  static RowMap make(const int64_t* n, int64_t rows) {
     const auto size = [](int64_t v) { return (uint32_t)(v > 0 ? v : 1); };
-    RowMap m{};
-    m.rows = m.places = (uint32_t)rows;
-    m.n1 = FastDiv::make(size(n[1]));
-    m.n2 = FastDiv::make(size(n[2]));
-    const int64_t a = (n[1] + 7) / 8, b = (n[2] + 7) / 8;
-    m.tiled = tiled && n[1] > 1 && n[2] > 1 && n[0] * a * b * 64 < 0x7fffffffLL - (1 << 20);
-    m.t1 = FastDiv::make(size(a));
-    m.t2 = FastDiv::make(size(b));
-    if (m.tiled) m.places = (uint32_t)(n[0] * a * b * 64);
-    return m;
+    return RowMap{(uint32_t)rows, FastDiv::make(size(n[1])), FastDiv::make(size(n[2]))};
   }
-  __device__ __forceinline__ RowIndex at(uint32_t place) const {
-    if (tiled) {
-      const uint32_t q = place >> 6, i = t2.div(q), i0 = t1.div(i);
-      return RowIndex{i0, (i - i0 * t1.d) * 8 + (place & 7), (q - i * t2.d) * 8 + (place >> 3 & 7)};
-    }
-    const uint32_t q = n2.div(place), i0 = n1.div(q);
-    return RowIndex{i0, q - i0 * n1.d, place - q * n2.d};
+  __device__ __forceinline__ RowIndex at(uint32_t row) const {
+    const uint32_t q = n2.div(row), i0 = n1.div(q);
+    return RowIndex{i0, q - i0 * n1.d, row - q * n2.d};
   }
 };
-// A place of that order and its row.
-template <bool DENSE>
-struct Spot {
-  uint32_t row;  // DENSE: the place
-  RowIndex i;    // not DENSE
-  bool live;     // there is a row
-  __device__ __forceinline__ RowIndex index(const RowMap& map) const {
-    if constexpr (DENSE)
-      return map.at(row);
-    else
-      return i;
-  }
-};
-
 __device__ __forceinline__ int64_t row_offset(const Strides3& s, uint32_t row, const RowMap& map, int dim) {
   if (s.dense) return (int64_t)row * dim;
   const RowIndex i = map.at(row);
@@ -387,37 +353,23 @@ struct Lanes {
   }
 };
 
-// The R places from `place` on.  Where rows are found by their index, lane r of a group finds that of place r
-// and hands it round: one search a lane instead of R.
-template <bool DENSE, int R, int VEC, int LPR, int NCH>
-__device__ __forceinline__ void spots(const Lanes<VEC, LPR, NCH>& l, const RowMap& map, uint32_t place, Spot<DENSE> (&s)[R]) {
-  if constexpr (DENSE) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      s[r].row = place + r;
-      s[r].live = place + r < map.places;
-    }
-  } else {
-    static_assert((R & (R - 1)) == 0 && (LPR || R == 1), "");
-    const uint32_t mine = place + (l.lane & (R - 1));
-    const RowIndex i = map.at(mine);
-    const bool live = mine < map.places && i.i1 < map.n1.d && i.i2 < map.n2.d;
-    const uint32_t row = live ? (i.i0 * map.n1.d + i.i1) * map.n2.d + i.i2 : ~0u;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if constexpr (R > 1) {
-        s[r].row = __shfl_sync(0xffffffffu, row, r, LPR);
-        s[r].i.i0 = __shfl_sync(0xffffffffu, i.i0, r, LPR);
-        s[r].i.i1 = __shfl_sync(0xffffffffu, i.i1, r, LPR);
-        s[r].i.i2 = __shfl_sync(0xffffffffu, i.i2, r, LPR);
-      } else {
-        s[r].row = row;
-        s[r].i = i;
-      }
-      s[r].live = s[r].row != ~0u;
+// R rows of a group that are worked on together, from `first` on.  DENSE: all tensors are dense, and a row's number
+// is all that is needed; else lane r of the group holds the index of row r.
+template <bool DENSE, int R>
+struct Batch {
+  uint32_t first, rows;
+  RowIndex mine;
+  template <class L>
+  __device__ __forceinline__ Batch(const L& l, const RowMap& map, uint32_t f) : first(f), rows(map.rows) {
+    if constexpr (!DENSE) {
+      static_assert((R & (R - 1)) == 0, "");
+      const uint32_t row = first + (R > 1 ? l.lane & (R - 1) : 0);
+      mine = map.at(row < rows ? row : rows - 1);
     }
   }
-}
+  __device__ __forceinline__ uint32_t row(int r) const { return first + r; }
+  __device__ __forceinline__ bool live(int r) const { return first + r < rows; }
+};
 
 // Rows of several warps: C pieces (of VEC channels) on `width` lanes, 16 channels a lane at most (registers); the
 // number of pieces a lane that leaves the fewest lanes idle, all but the last full.
@@ -445,27 +397,35 @@ __host__ __device__ constexpr int row_slot(int width, int dim) {
   return VEC > 1 ? width * NCH * VEC * (int)sizeof(T) : (dim * (int)sizeof(T) + 15) / 16 * 16 + 16;
 }
 
-// A tensor's rows.  DENSE: row after row, so that a row's address is one multiply-add; else by strides.
-template <class T, bool DENSE>
+// A tensor's rows.  A dense one's row is found by one multiply-add; of a strided one lane r of a group works out where
+// row r lies, and hands it round (every lane of a warp takes part).
+template <class T, int LPR, bool DENSE>
 struct RowsOf {
   char* base;
-  uint32_t pitch;  // bytes of a row (DENSE)
+  uint32_t pitch;  // bytes of a dense row
+  bool dense;
   int64_t s0, s1, s2;
   __device__ __forceinline__ RowsOf(const void* p, const Strides3& s, int dim, int lane_elements) {
     base = static_cast<char*>(const_cast<void*>(p)) + lane_elements * (int)sizeof(T);
-    if constexpr (DENSE) {
-      pitch = dim * (uint32_t)sizeof(T);
-    } else {
+    pitch = dim * (uint32_t)sizeof(T);
+    if constexpr (!DENSE) {
+      dense = s.dense;
       s0 = s.s[0] * (int)sizeof(T);
       s1 = s.s[1] * (int)sizeof(T);
       s2 = s.s[2] * (int)sizeof(T);
     }
   }
-  __device__ __forceinline__ T* at(const Spot<DENSE>& p) const {
-    if constexpr (DENSE)
-      return reinterpret_cast<T*>(base + (uint64_t)p.row * pitch);
-    else
-      return reinterpret_cast<T*>(base + s0 * p.i.i0 + s1 * p.i.i1 + s2 * p.i.i2);
+  template <int R>
+  __device__ __forceinline__ void at(const Batch<DENSE, R>& batch, T* (&p)[R]) const {
+    if (DENSE || dense) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) p[r] = reinterpret_cast<T*>(base + (uint64_t)batch.row(r) * pitch);
+    } else {
+      const int64_t off = s0 * batch.mine.i0 + s1 * batch.mine.i1 + s2 * batch.mine.i2;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        p[r] = reinterpret_cast<T*>(base + (R > 1 ? __shfl_sync(0xffffffffu, off, r, LPR ? LPR : 32) : off));
+    }
   }
 };
 
@@ -477,7 +437,7 @@ struct RowIn {
   static constexpr int B = VEC * sizeof(T);
   static_assert(VEC == 1 || B == 8 || B == 16, "");
   const L& l;
-  RowsOf<T, DENSE> rows;
+  RowsOf<T, LPR, DENSE> rows;
   char* ring;  // VEC > 1: at the lane's first piece
   uint32_t ring32;
   __device__ __forceinline__ RowIn(const L& l_, const void* p, const Strides3& s, char* r)
@@ -496,8 +456,8 @@ struct RowIn {
       }
     }
   }
-  __device__ __forceinline__ void issue(int off, const Spot<DENSE>& spot) const {
-    const T* p = rows.at(spot);
+  // row p = rows.at(...)
+  __device__ __forceinline__ void issue(int off, const T* p) const {
     if constexpr (VEC > 1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c)
@@ -521,7 +481,7 @@ struct RowIn {
         copy_zero<16>(ring32 + off + i, rows.base);
     }
   }
-  __device__ __forceinline__ void read(int off, const Spot<DENSE>& spot, Pair (&x)[L::PAIRS]) const {
+  __device__ __forceinline__ void read(int off, const T* row, Pair (&x)[L::PAIRS]) const {
     if constexpr (VEC > 1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
@@ -530,7 +490,7 @@ struct RowIn {
         for (int j = 0; j < VEC / 2; ++j) x[c * VEC / 2 + j] = to_pair(p.v + 2 * j);
       }
     } else {
-      const T* p = reinterpret_cast<const T*>(ring + off + (reinterpret_cast<uintptr_t>(rows.at(spot)) & 15));
+      const T* p = reinterpret_cast<const T*>(ring + off + (reinterpret_cast<uintptr_t>(row) & 15));
       float v[2 * L::PAIRS];
 #pragma unroll
       for (int c = 0; c < 2 * L::PAIRS; ++c) v[c] = c < NCH && l.act(c) ? to_f32(p[l.col(c)]) : 0.0f;
@@ -544,10 +504,9 @@ template <class T, int VEC, int LPR, int NCH, bool DENSE>
 struct RowOut {
   using L = Lanes<VEC, LPR, NCH>;
   const L& l;
-  RowsOf<T, DENSE> rows;
+  RowsOf<T, LPR, DENSE> rows;
   __device__ __forceinline__ RowOut(const L& l_, const void* p, const Strides3& s) : l(l_), rows(p, s, l_.dim, l_.lane * VEC) {}
-  __device__ __forceinline__ T* at(const Spot<DENSE>& spot) const { return rows.at(spot); }
-  // piece c of a row's values, if the lane has it; p = at(its spot)
+  // piece c of a row's values, if the lane has it; p = rows.at(...)
   __device__ __forceinline__ void piece(T* p, int c, const Pair (&x)[L::PAIRS]) const {
     if (!l.act(c)) return;
     if constexpr (VEC > 1) {
@@ -560,8 +519,7 @@ struct RowOut {
       p[c * l.width] = from_f32<T>(c & 1 ? h.y : h.x);
     }
   }
-  __device__ __forceinline__ void row(const Spot<DENSE>& spot, const Pair (&x)[L::PAIRS]) const {
-    T* p = at(spot);
+  __device__ __forceinline__ void row(T* p, const Pair (&x)[L::PAIRS]) const {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) piece(p, c, x);
   }

@@ -63,30 +63,34 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
 
   const RowMap& map = a.map;
   const uint32_t step = l.groups * R;
+  using Rows = Batch<DENSE, R>;
   const auto issue = [&](uint32_t base, int s) {
-    Spot<DENSE> spot[R];
-    spots(l, map, base + l.group * R, spot);
+    const Rows batch(l, map, base + l.group * R);
+    TX *px[R], *ps[R];
+    TO* po[R];
+    x.rows.at(batch, px);
+    dout.rows.at(batch, po);
+    if constexpr (HASY) ds.rows.at(batch, ps);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (!spot[r].live) {  // adds nothing to the column sums
+      if (!batch.live(r)) {  // adds nothing to the column sums
         x.issue_none(s * stage + r * slot_x);
         dout.issue_none(s * stage + r * slot_o);
         continue;
       }
-      x.issue(s * stage + r * slot_x, spot[r]);
-      dout.issue(s * stage + r * slot_o, spot[r]);
+      x.issue(s * stage + r * slot_x, px[r]);
+      dout.issue(s * stage + r * slot_o, po[r]);
       if constexpr (HASY)
-        if (has_ds) ds.issue(s * stage + r * slot_x, spot[r]);
+        if (has_ds) ds.issue(s * stage + r * slot_x, ps[r]);
     }
   };
   float mean_next[R], rstd_next[R];  // of the next batch
-  Spot<DENSE> next[R];
   const auto statistics = [&](uint32_t base) {
-    spots(l, map, base + l.group * R, next);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      mean_next[r] = next[r].live ? a.mean[next[r].row] : 0.0f;
-      rstd_next[r] = next[r].live ? a.rstd[next[r].row] : 0.0f;
+      const uint32_t row = base + l.group * R + r;
+      mean_next[r] = row < map.rows ? a.mean[row] : 0.0f;
+      rstd_next[r] = row < map.rows ? a.rstd[row] : 0.0f;
     }
   };
 
@@ -106,23 +110,29 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     if (ahead < end) issue(ahead, s == 0 ? S - 1 : s - 1);
     copy_commit();
     float mean[R], rstd[R];
-    Spot<DENSE> spot[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      spot[r] = next[r];
       mean[r] = mean_next[r];
       rstd[r] = rstd_next[r];
     }
     statistics(base + step);
     copy_wait<S - 1>();
     l.sync();
+    const Rows batch(l, map, base + l.group * R);
+    TX *px[R], *ps[R];
+    TO* po[R];
+    if constexpr (VEC == 1) {
+      x.rows.at(batch, px);
+      dout.rows.at(batch, po);
+      if constexpr (HASY) ds.rows.at(batch, ps);
+    }
     // v[2 r] = sum g, v[2 r + 1] = sum g xh
     Pair xh[R][P], g[R][P];
     float v[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      x.read(s * stage + r * slot_x, spot[r], xh[r]);
-      dout.read(s * stage + r * slot_o, spot[r], g[r]);
+      x.read(s * stage + r * slot_x, VEC == 1 ? px[r] : nullptr, xh[r]);
+      dout.read(s * stage + r * slot_o, VEC == 1 ? po[r] : nullptr, g[r]);
       const Pair q = both(rstd[r]), mq = both(-mean[r] * rstd[r]);
       Pair s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
@@ -138,18 +148,16 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
       v[2 * r + 1] = total(s2);
     }
     l.sum(v, red, phase);
+    TX* pdx[R];
+    TY* pdy[R];
+    const Batch<true, R> written(l, map, batch.first);
+    dx.rows.at(written, pdx);
+    dy.rows.at(written, pdy);
     uint32_t whole = ~0u;  // bit r: row r is not dropped whole
     if constexpr (HASY) {
       if (row_draw) {
-        const int mine = LPR ? l.lane & (R - 1) : 0;
-        RowIndex i = spot[0].index(map);
-        if constexpr (DENSE)
-          i = map.at(spot[0].row + mine);
-        else
-#pragma unroll
-          for (int r = 1; r < R; ++r)
-            if (r == mine) i = spot[r].i;
-        const bool k = rng.word(mask_base(a.drop, i)) > a.drop.drop_max;
+        const uint32_t mine = batch.first + (LPR ? l.lane & (R - 1) : 0);
+        const bool k = rng.word(mask_base(a.drop, map.at(mine))) > a.drop.drop_max;
         whole = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -158,8 +166,7 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool live = spot[r].live;
-      const Spot<true> to{spot[r].row, {}, live};
+      const bool live = batch.live(r);
       const float t = -inv_d * rstd[r];
       const Pair c1 = both(v[2 * r] * t), c2 = both(v[2 * r + 1] * t), q = both(rstd[r]);
 #pragma unroll
@@ -167,16 +174,16 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
       if constexpr (HASY) {
         if (has_ds) {
           Pair sv[P];
-          ds.read(s * stage + r * slot_x, spot[r], sv);
+          ds.read(s * stage + r * slot_x, VEC == 1 ? ps[r] : nullptr, sv);
 #pragma unroll
           for (int j = 0; j < P; ++j) g[r][j] = g[r][j] + sv[j];
         }
       }
-      if (a.dx && live) dx.row(to, g[r]);
+      if (a.dx && live) dx.row(pdx[r], g[r]);
       if constexpr (HASY) {
         if (has_dy) {
           if (draw) {
-            each_kept(l, rng, mask_base(a.drop, spot[r].index(map)), a.drop.drop_max, [&](bool k, int i) {
+            each_kept(l, rng, mask_base(a.drop, map.at(batch.row(r))), a.drop.drop_max, [&](bool k, int i) {
               const float2 gi = halves(g[r][i / 2]);
               const float f = k ? (i & 1 ? gi.y : gi.x) * a.drop.scale : 0.0f;
               g[r][i / 2] = i & 1 ? pair(gi.x, f) : pair(f, gi.y);
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
 #pragma unroll
             for (int j = 0; j < P; ++j) g[r][j] = whole >> r & 1 ? g[r][j] * scale : both(0.0f);
           }
-          if (live) dy.row(to, g[r]);
+          if (live) dy.row(pdy[r], g[r]);
         }
       }
     }
@@ -309,7 +316,7 @@ cudaError_t bwd_one(const NormBwdArgs& a, int width, int threads, cudaStream_t s
       e != cudaSuccess)
     return e;
   if (fit > kCtasPerSm) fit = kCtasPerSm;
-  const uint32_t per = groups * R, batches = (a.map.places + per - 1) / per;
+  const uint32_t per = groups * R, batches = (a.map.rows + per - 1) / per;
   const Split split = share(batches, (uint32_t)(device_sm_count() * fit), per);
   const uint32_t grid = split.big + (split.few ? (batches - split.big * split.many + split.few - 1) / split.few : 0);
   norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE><<<grid, threads, smem, st>>>(a, width, split);

@@ -35,7 +35,6 @@ struct Shape {
   int dim;
   int64_t rows;
   int vec;
-  bool transposed = false;  // some tensor lies with its last two leading axes swapped
 
   int init(const char* name, const int64_t* shape, int64_t d, int64_t max_dim) {
     what = name;
@@ -68,7 +67,7 @@ struct Shape {
     while (dim % vec) vec = vec == 8 ? 4 : 1;
     return TRIATTN_OK;
   }
-  RowMap map(bool tiles = false) const { return RowMap::make(n, rows, tiles && transposed); }
+  RowMap map() const { return RowMap::make(n, rows); }
   // A tensor of this shape: its strides (NULL = dense), and what they and its address allow.  `written`:
   // no two rows may share memory.
   int tensor(const char* name, const void* p, int dtype, const int64_t* strides, Strides3* out, bool written) {
@@ -102,7 +101,6 @@ struct Shape {
       if (ok) break;
       vec = vec == 8 ? 4 : 1;
     }
-    if (n[1] > 1 && n[2] > 1 && s.s[1] < s.s[2] && s.s[1] > 0) transposed = true;
     *out = s;
     return TRIATTN_OK;
   }
@@ -170,7 +168,7 @@ int triattn_layer_norm(const void* x, int x_dtype, const int64_t* x_strides, con
   NormFwdArgs a{};
   if (int r = s.tensor("x", x, x_dtype, x_strides, &a.zs, false)) return r;
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
-  a.z = x; a.out = out; a.map = s.map(true); a.dim = s.dim;
+  a.z = x; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
   a.mean = mean; a.rstd = rstd;
   return finish(launch_norm_fwd(a, x_dtype, out_dtype, s.vec, static_cast<cudaStream_t>(stream)), what);
@@ -229,7 +227,7 @@ int triattn_dropout_add_layer_norm(const void* z, int z_dtype, const int64_t* z_
   if (int r = s.tensor("y", y, y_dtype, y_strides, &a.ys, false)) return r;
   if (int r = s.tensor("sum", sum, z_dtype, sum_strides, &a.ss, true)) return r;
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
-  a.z = z; a.y = y; a.sum = sum; a.out = out; a.map = s.map(true); a.dim = s.dim;
+  a.z = z; a.y = y; a.sum = sum; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
   a.mean = mean; a.rstd = rstd;
   return finish(launch_fused_fwd(a, z_dtype, y_dtype, out_dtype, s.vec, static_cast<cudaStream_t>(stream)), what);
@@ -283,7 +281,7 @@ int triattn_layer_norm_backward(const void* dout, int dout_dtype, const int64_t*
   if (dy)
     if (int r = s.tensor("dy", dy, y_dtype, nullptr, &dense, true)) return r;
   if (!dx && !dy && !dweight && !dbias) return TRIATTN_OK;
-  a.dout = dout; a.x = x; a.ds = dsum; a.map = s.map(true); a.dim = s.dim;
+  a.dout = dout; a.x = x; a.ds = dsum; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.param_dtype = param_dtype; a.mean = mean; a.rstd = rstd;
   a.dx = dx; a.dy = dy; a.dweight = dweight; a.dbias = dbias;
   a.partial = dweight || dbias ? static_cast<float*>(workspace) : nullptr;

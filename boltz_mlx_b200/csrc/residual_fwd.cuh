@@ -67,21 +67,18 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
 
   const RowMap& map = a.map;
   const uint32_t step = l.groups * R;
+  using Rows = Batch<DENSE, R>;
   const auto issue = [&](uint32_t base, int s) {
-    Spot<DENSE> spot[R];
-    spots(l, map, base + l.group * R, spot);
+    const Rows batch(l, map, base + l.group * R);
+    TX* pz[R];
+    TY* py[R];
+    if constexpr (HASX) z.rows.at(batch, pz);
+    if constexpr (HASY) y.rows.at(batch, py);
     if constexpr (HASY) {
       if (row_draw) {
         // one draw per row: lane r of a group takes that of row r, and hands it round
-        const int mine = LPR ? l.lane & (R - 1) : 0;
-        RowIndex i = spot[0].index(map);
-        if constexpr (DENSE)
-          i = map.at(spot[0].row + mine);
-        else
-#pragma unroll
-          for (int r = 1; r < R; ++r)
-            if (r == mine) i = spot[r].i;
-        const bool k = rng.word(mask_base(a.drop, i)) > a.drop.drop_max;
+        const uint32_t mine = batch.first + (LPR ? l.lane & (R - 1) : 0);
+        const bool k = rng.word(mask_base(a.drop, map.at(mine))) > a.drop.drop_max;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const uint32_t bit = 1u << (s * R + r);
@@ -91,13 +88,13 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (!spot[r].live) continue;
+      if (!batch.live(r)) continue;
       // of a row that is dropped whole, y is not read, nor, in place, z
       const bool keep = !HASY || (kept >> (s * R + r) & 1);
       if constexpr (HASX)
-        if (keep || !(DO == kAdd && a.in_place)) z.issue(s * stage + r * slot_x, spot[r]);
+        if (keep || !(DO == kAdd && a.in_place)) z.issue(s * stage + r * slot_x, pz[r]);
       if constexpr (HASY)
-        if (keep) y.issue(s * stage + r * slot_y, spot[r]);
+        if (keep) y.issue(s * stage + r * slot_y, py[r]);
     }
   };
 
@@ -118,14 +115,18 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
     copy_commit();
     copy_wait<S - 1>();
     l.sync();
-    Spot<DENSE> spot[R];
-    spots(l, map, base + l.group * R, spot);
-    // Places without a row are computed from what their slot holds, and not stored.
+    const Rows batch(l, map, base + l.group * R);
+    TX *pz[R], *ps[R];
+    TY* py[R];
+    if constexpr (HASX && VEC == 1) z.rows.at(batch, pz);
+    if constexpr (HASY && VEC == 1) y.rows.at(batch, py);
+    if constexpr (HASY) sum.rows.at(batch, ps);
+    // Rows behind the last one are computed from what their slot holds, and not stored.
     Pair x[R][P];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if constexpr (HASX) {
-        z.read(s * stage + r * slot_x, spot[r], x[r]);
+        z.read(s * stage + r * slot_x, VEC == 1 ? pz[r] : nullptr, x[r]);
       } else {
 #pragma unroll
         for (int j = 0; j < P; ++j) x[r][j] = both(0.0f);
@@ -134,9 +135,9 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
         const bool whole = kept >> (s * R + r) & 1;
         if (whole) {
           Pair v[P];
-          y.read(s * stage + r * slot_y, spot[r], v);
+          y.read(s * stage + r * slot_y, VEC == 1 ? py[r] : nullptr, v);
           if (draw) {
-            each_kept(l, rng, mask_base(a.drop, spot[r].index(map)), a.drop.drop_max, [&](bool k, int i) {
+            each_kept(l, rng, mask_base(a.drop, map.at(batch.row(r))), a.drop.drop_max, [&](bool k, int i) {
               const float2 xi = halves(x[r][i / 2]), vi = halves(v[i / 2]);
               const float f = i & 1 ? xi.y : xi.x, g = k ? fmaf(i & 1 ? vi.y : vi.x, a.drop.scale, f) : f;
               x[r][i / 2] = i & 1 ? pair(xi.x, g) : pair(g, xi.y);
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
             x[r][j] = to_pair(held);
           }
         }
-        if (spot[r].live && (whole || !(DO == kAdd && a.in_place))) sum.row(spot[r], x[r]);
+        if (batch.live(r) && (whole || !(DO == kAdd && a.in_place))) sum.row(ps[r], x[r]);
       }
     }
     l.sync();
@@ -183,14 +184,13 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
       if (a.mean && l.lane == 0) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
-          if (spot[r].live) {
-            a.mean[spot[r].row] = mean[r];
-            a.rstd[spot[r].row] = var[r];
+          if (batch.live(r)) {
+            a.mean[batch.row(r)] = mean[r];
+            a.rstd[batch.row(r)] = var[r];
           }
       }
       TO* po[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) po[r] = out.at(spot[r]);
+      out.rows.at(batch, po);
       constexpr int STEP = VEC == 1 && NCH > 1 ? 2 : 1;  // pieces of a pair
 #pragma unroll
       for (int c = 0; c < NCH; c += STEP) {
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
             Pair& h = x[r][(VEC > 1 ? c * N : c / 2) + j];
             h = fma2(h * rstd, wc[j], bc[j]);
           }
-          if (spot[r].live) {
+          if (batch.live(r)) {
 #pragma unroll
             for (int k = 0; k < STEP; ++k)
               if (c + k < NCH) out.piece(po[r], c + k, x[r]);
@@ -248,7 +248,7 @@ cudaError_t fwd_one(const NormFwdArgs& a, int width, int threads, cudaStream_t s
   // CTA leaves the SMs that the memory system serves last working alone at the end (0.82 of the copy rate
   // instead of 0.98 at 2^20 rows of 128 fp32).  A CTA has to load weight and bias, though, so that long rows
   // want more batches, in 16 bits (half the traffic a row) most (0.70 instead of 0.62 at 8192 rows of 4096).
-  const uint32_t per = groups * R, batches = (a.map.places + per - 1) / per;
+  const uint32_t per = groups * R, batches = (a.map.rows + per - 1) / per;
   const uint32_t resident = (uint32_t)(device_sm_count() * fit);
   uint32_t few = (batches + resident - 1) / resident;
   constexpr uint32_t most = LPR ? 5 : VEC == 8 ? 16 : 4;
