@@ -177,11 +177,7 @@ cudaError_t launch_types(const DropoutAddArgs& a, int vec, cudaStream_t st) {
   const auto aligned = [](const void* p, size_t b) { return reinterpret_cast<uintptr_t>(p) % b == 0; };
   const bool flat = (!a.z || a.zs.dense) && a.ys.dense && a.os.dense && aligned(a.z, FULL * sizeof(TZ)) &&
                     aligned(a.y, FULL * sizeof(TY)) && aligned(a.out, FULL * sizeof(TO));
-  const int64_t m2 = a.dim, m1 = m2 * a.map.n2.d, m0 = m1 * a.map.n1.d;
-  const bool own = !a.drop.on || (a.drop.per_channel && (a.map.n2.d == 1 || a.drop.m[2] == m2) &&
-                                  (a.map.n1.d == 1 || a.drop.m[1] == m1) &&
-                                  (a.map.rows == a.map.n1.d * a.map.n2.d || a.drop.m[0] == m0));
-  if (flat && own) return launch_one<TZ, TY, TO, FULL, kVector, HASZ>(a, st);
+  if (flat && a.vector) return launch_one<TZ, TY, TO, FULL, kVector, HASZ>(a, st);
   if (vec >= FULL) return launch_one<TZ, TY, TO, FULL, kRows, HASZ>(a, st);
   if (flat) return launch_one<TZ, TY, TO, FULL, kMixed, HASZ>(a, st);
   return launch_one<TZ, TY, TO, 1, kRows, HASZ>(a, st);

@@ -61,39 +61,59 @@ __device__ __forceinline__ int64_t row_offset(const Strides3& s, uint32_t row, c
   return s.s[0] * i.i0 + s.s[1] * i.i1 + s.s[2] * i.i2;
 }
 
+constexpr uint32_t PHILOX_M0 = 0xD2511F53u, PHILOX_M1 = 0xCD9E8D57u;  // multipliers of Philox4x32
+constexpr uint32_t PHILOX_W0 = 0x9E3779B9u, PHILOX_W1 = 0xBB67AE85u;  // steps of its key
+
 // ---- the keep mask ------------------------------------------------------------------------------
 struct Dropout {
   int on;                // 0: everything is kept and scale is 1
   uint32_t drop_max;     // a word u is dropped if u <= drop_max
   float scale;
-  uint64_t seed, offset;
+  uint64_t offset;
+  uint32_t key[10][2];    // the ten rounds' keys, from the seed
   const uint64_t* state;  // device {seed, offset} instead of the two above, or nullptr
   int64_t m[3];           // strides of the mask tensor's leading axes, 0 where shared
   int per_channel;        // 1: every channel has its own position, 0: one for the whole row
 };
 
+// The generator of one launch.  The rounds' keys are operands from the kernel's parameters where the host knows the
+// seed; where the device holds it, they are worked out as they are used (20 more instructions a block of 60).
 struct Philox {
+  const Dropout& d;
   uint32_t k0, k1, o0, o1;
-  __device__ __forceinline__ explicit Philox(const Dropout& d) {
-    const uint64_t seed = d.state ? d.state[0] : d.seed, offset = d.state ? d.state[1] : d.offset;
-    k0 = (uint32_t)seed;
-    k1 = (uint32_t)(seed >> 32);
+  __device__ __forceinline__ explicit Philox(const Dropout& drop) : d(drop) {
+    k0 = k1 = 0;
+    uint64_t offset = d.offset;
+    if (d.state) {
+      k0 = (uint32_t)d.state[0];
+      k1 = (uint32_t)(d.state[0] >> 32);
+      offset = d.state[1];
+    }
     o0 = (uint32_t)offset;
     o1 = (uint32_t)(offset >> 32);
+  }
+  static __device__ __forceinline__ void round(uint32_t& c0, uint32_t& c1, uint32_t& c2, uint32_t& c3, uint32_t a, uint32_t b) {
+    const uint64_t p = (uint64_t)PHILOX_M0 * c0, q = (uint64_t)PHILOX_M1 * c2;
+    c0 = (uint32_t)(q >> 32) ^ c1 ^ a;
+    c1 = (uint32_t)q;
+    c2 = (uint32_t)(p >> 32) ^ c3 ^ b;
+    c3 = (uint32_t)p;
   }
   // the four words of block (positions 4 * block .. 4 * block + 3); Salmon, Moraes, Dror, Shaw,
   // Parallel random numbers: as easy as 1, 2, 3 (2011), 10 rounds
   __device__ __forceinline__ uint4 block(uint64_t block) const {
-    uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = o0, c3 = o1, a = k0, b = k1;
+    uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = o0, c3 = o1;
+    if (!d.state) {
 #pragma unroll
-    for (int r = 0; r < 10; ++r) {
-      const uint64_t p = (uint64_t)0xD2511F53u * c0, q = (uint64_t)0xCD9E8D57u * c2;
-      c0 = (uint32_t)(q >> 32) ^ c1 ^ a;
-      c1 = (uint32_t)q;
-      c2 = (uint32_t)(p >> 32) ^ c3 ^ b;
-      c3 = (uint32_t)p;
-      a += 0x9E3779B9u;
-      b += 0xBB67AE85u;
+      for (int r = 0; r < 10; ++r) round(c0, c1, c2, c3, d.key[r][0], d.key[r][1]);
+    } else {
+      uint32_t a = k0, b = k1;
+#pragma unroll
+      for (int r = 0; r < 10; ++r) {
+        round(c0, c1, c2, c3, a, b);
+        a += PHILOX_W0;
+        b += PHILOX_W1;
+      }
     }
     return make_uint4(c0, c1, c2, c3);
   }
@@ -391,6 +411,14 @@ RowWidth row_width(int C, int threads) {  // a CTA of about so many threads
   return best;
 }
 
+// What Lanes::act takes for granted: the pieces that are always there are, and the others reach the row's end.  Every
+// launch asks.
+template <int VEC, int NCH>
+bool pieces_fit(int dim, int width) {
+  const int always = VEC > 1 ? NCH - 1 : NCH - 4;
+  return always * width * VEC <= dim && NCH * width * VEC >= dim && dim % VEC == 0;
+}
+
 // Bytes of shared memory that one row of a tensor takes in one stage, per row's group of lanes.
 template <class T, int VEC, int NCH>
 __host__ __device__ constexpr int row_slot(int width, int dim) {
@@ -674,6 +702,7 @@ struct DropoutAddArgs {
   RowMap map;
   int dim;
   int in_place;  // out is z: what is dropped whole is neither read nor written
+  int vector;    // the tensors are one long vector each, and so is the mask
   Dropout drop;
 };
 
@@ -730,7 +759,7 @@ cudaError_t launch_fused_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int
 cudaError_t launch_fused16_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int dout_dtype, int vec, cudaStream_t st);
 cudaError_t launch_dropout_add(const DropoutAddArgs& a, int z_dtype, int y_dtype, int out_dtype, int vec,
                                cudaStream_t st);
-// triattn_dropout_add over dense rows of which each is dropped or kept whole; vec 4 or 8, dim up to 64 vec (128 for 4)
+// triattn_dropout_add by rows, dim up to 512
 cudaError_t launch_dropout_rows(const NormFwdArgs& a, int y_dtype, int out_dtype, int vec, cudaStream_t st);
 int norm_bwd_max_ctas();  // of a launch: rows of its partial sums
 

@@ -308,6 +308,7 @@ Split share(uint32_t batches, uint32_t resident, uint32_t per) {
 template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, bool HASY, bool DENSE>
 cudaError_t bwd_one(const NormBwdArgs& a, int width, int threads, cudaStream_t st) {
   static KernelInfo info;
+  if (!pieces_fit<VEC, NCH>(a.dim, width)) return cudaErrorInvalidConfiguration;
   const int groups = threads / width, sets = LPR ? threads / 32 : groups;
   size_t smem = (size_t)groups * S * bwd_stage_bytes<TX, TO, VEC, NCH, R, HASY>(width, a.dim);
   if (const size_t sums = (size_t)sets * 2 * a.dim * 4; sets > 1 && smem < sums) smem = sums;

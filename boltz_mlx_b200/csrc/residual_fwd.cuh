@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_fwd_kernel(const NormFwd
 template <class TX, class TY, class TO, int VEC, int LPR, int NCH, int R, int S, Does DO, bool DENSE>
 cudaError_t fwd_one(const NormFwdArgs& a, int width, int threads, cudaStream_t st) {
   static KernelInfo info;
+  if (!pieces_fit<VEC, NCH>(a.dim, width)) return cudaErrorInvalidConfiguration;
   const int groups = threads / width, wb = DO == kNorm || DO == kFused ? LPR * VEC * NCH * 8 : 0;
   const size_t smem = wb + (size_t)groups * S * fwd_stage_bytes<TX, TY, VEC, NCH, R, DO>(width, a.dim);
   int fit = 0;

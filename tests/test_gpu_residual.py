@@ -139,6 +139,32 @@ def test_layer_norm_and_gradients(tx, to, dim):
         close(db, rb, tb, F, f"db {rows} {dim}")
 
 
+@pytest.mark.parametrize("tx,to", [(F, B), (H, H)])
+def test_layer_norm_every_width(tx, to):
+    """A row's lanes and pieces change with the width: all widths up to 140, and every 13th to 2100."""
+    for dim in [*range(1, 140), *range(140, 2100, 13), *range(248, 2100, 248), 3000, 5000, 6000, 7777]:
+        x, w = normal((3, dim), tx, dim).requires_grad_(), normal((dim,), F, dim + 1, 1.0, 0.2).requires_grad_()
+        dh = normal((3, dim), to, dim + 3)
+        r = Row(x, w, None)
+        h = layer_norm(x, w, out_dtype=to)
+        inside(h, r.h, r.tol_h(to), f"h {dim}")
+        (rx, rw, _), (tx_, tw, _) = r.grads(dh)
+        dx, dw = torch.autograd.grad(h, (x, w), dh)
+        close(dx, rx, tx_, tx, f"dx {dim}")
+        close(dw, rw, tw, F, f"dw {dim}")
+
+
+@pytest.mark.parametrize("tz,ty", [(F, F), (F, B), (H, H)])
+def test_dropout_every_width(tz, ty):
+    for dim in [*range(1, 70), *range(70, 600, 11), *range(96, 1100, 96)]:
+        z, y = normal((5, dim), tz, 1), normal((5, dim), ty, 2)
+        for share in ((), (0,), (1,)):
+            ref = rounded(dropout_add_ref(f64(z), f64(y), 0.4, 3, 1, share), tz)
+            assert torch.equal(dropout_add(z, y, 0.4, 3, 1, share=share), ref), (dim, share)
+            s, _ = dropout_add_layer_norm(z, y, None, None, 0.4, 3, 1, share=share)
+            assert torch.equal(s, ref), (dim, share)
+
+
 @pytest.mark.parametrize("dim", [128, 131, 1024])
 def test_layer_norm_many_rows(dim):
     """More rows than one sweep of the grid, not a multiple of anything; the same bits on every run."""
@@ -276,7 +302,7 @@ SHARES = [(), (2, 3), (1, 3), (1,), (0, 1, 2), (3,), (0, 1, 2, 3), (0,)]
 
 @pytest.mark.parametrize("tz,ty", [(F, F), (F, H), (F, B), (H, H), (B, B)])
 @pytest.mark.parametrize("share", SHARES)
-@pytest.mark.parametrize("dim", [1, 3, 8, 33, 128, 1000])
+@pytest.mark.parametrize("dim", [1, 3, 8, 33, 128, 129, 200, 264, 300, 333, 400, 510, 512, 1000])
 def test_dropout_add(tz, ty, share, dim):
     shape, p, seed, offset = (2, 5, 7, dim), 0.3, 0xDEADBEEF12345678, (1 << 40) + 5
     z, y, g = normal(shape, tz, 1), normal(shape, ty, 2), normal(shape, tz, 3)
