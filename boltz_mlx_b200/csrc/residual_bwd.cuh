@@ -204,7 +204,6 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
 
   if (!a.partial) return;
   // groups of one warp first (they own the same channels), then all groups through shared memory
-  float* part = a.partial + (size_t)blockIdx.x * 2 * D;
 #pragma unroll
   for (int o = LPR ? LPR : 32; o < 32; o <<= 1) {
 #pragma unroll
@@ -214,10 +213,10 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     }
   }
   const int sets = LPR ? blockDim.x >> 5 : l.groups;
-  const bool writes = LPR ? (threadIdx.x & 31) < LPR : true;
-  float* mine = sets == 1 ? part : reinterpret_cast<float*>(smem) + (size_t)(LPR ? threadIdx.x >> 5 : l.group) * 2 * D;
+  float* sums = reinterpret_cast<float*>(smem);
+  float* mine = sums + (size_t)(LPR ? threadIdx.x >> 5 : l.group) * 2 * D;
   __syncthreads();  // every warp has read its last rows
-  if (writes) {
+  if (!LPR || (threadIdx.x & 31) < LPR) {
 #pragma unroll
     for (int i = 0; i < L::EPL; ++i) {
       if (!l.act(i / VEC)) continue;
@@ -226,12 +225,24 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
       mine[D + l.col(i / VEC) + i % VEC] = i & 1 ? t.y : t.x;
     }
   }
-  if (sets == 1) return;
   __syncthreads();
+  float* part = a.partial + (size_t)blockIdx.x * 2 * D;
   for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
     float t = 0.0f;
-    for (int k = 0; k < sets; ++k) t += reinterpret_cast<const float*>(smem)[(size_t)k * 2 * D + i];
-    part[i] = t;
+    for (int k = 0; k < sets; ++k) t += sums[(size_t)k * 2 * D + i];
+    if (gridDim.x > 1) {
+      part[i] = t;
+    } else {  // the only CTA's sums are the gradients
+      void* grad = i < D ? a.dweight : a.dbias;
+      const int c = i < D ? i : i - D;
+      if (!grad) continue;
+      if (a.param_dtype == DT_F32)
+        static_cast<float*>(grad)[c] = t;
+      else if (a.param_dtype == DT_F16)
+        static_cast<__half*>(grad)[c] = from_f32<__half>(t);
+      else
+        static_cast<__nv_bfloat16*>(grad)[c] = from_f32<__nv_bfloat16>(t);
+    }
   }
 }
 
@@ -293,7 +304,9 @@ cudaError_t launch_join(const NormBwdArgs& a, int ctas, cudaStream_t st) {
 // and read), so a share has kRows rows at least, or there is one kind of CTA only.  What a CTA adds up goes by
 // its index, not by when it runs.
 constexpr uint32_t kRows = 64;
+constexpr uint32_t kAlone = 4;  // so few batches one CTA works off alone, and needs no second kernel to add up
 Split share(uint32_t batches, uint32_t resident, uint32_t per) {
+  if (batches <= kAlone) return Split{1, batches, 0, batches};
   Split s{resident, batches / 4 * 3 / resident, 0, batches};
   s.few = s.many / 8;
   if (s.few * per < kRows) s.few = (kRows + per - 1) / per;
@@ -311,7 +324,7 @@ cudaError_t bwd_one(const NormBwdArgs& a, int width, int threads, cudaStream_t s
   if (!pieces_fit<VEC, NCH>(a.dim, width)) return cudaErrorInvalidConfiguration;
   const int groups = threads / width, sets = LPR ? threads / 32 : groups;
   size_t smem = (size_t)groups * S * bwd_stage_bytes<TX, TO, VEC, NCH, R, HASY>(width, a.dim);
-  if (const size_t sums = (size_t)sets * 2 * a.dim * 4; sets > 1 && smem < sums) smem = sums;
+  if (const size_t sums = (size_t)sets * 2 * a.dim * 4; smem < sums) smem = sums;
   int fit = 0;
   if (cudaError_t e = info.fit(norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE>, threads, smem, &fit);
       e != cudaSuccess)
@@ -321,7 +334,7 @@ cudaError_t bwd_one(const NormBwdArgs& a, int width, int threads, cudaStream_t s
   const Split split = share(batches, (uint32_t)(device_sm_count() * fit), per);
   const uint32_t grid = split.big + (split.few ? (batches - split.big * split.many + split.few - 1) / split.few : 0);
   norm_bwd_kernel<TX, TY, TO, VEC, LPR, NCH, R, S, HASY, DENSE><<<grid, threads, smem, st>>>(a, width, split);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess || !a.partial) return e;
+  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess || !a.partial || grid == 1) return e;
   if (a.param_dtype == DT_F32) return launch_join<float>(a, (int)grid, st);
   if (a.param_dtype == DT_F16) return launch_join<__half>(a, (int)grid, st);
   return launch_join<__nv_bfloat16>(a, (int)grid, st);

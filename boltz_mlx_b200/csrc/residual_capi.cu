@@ -222,6 +222,20 @@ int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, co
     return finish(launch_dropout_rows(f, y_dtype, out_dtype, s.vec, static_cast<cudaStream_t>(stream)), what);
   }
   a.vector = is_vector(a);
+  // A 16-bit vector goes by rows, too, cut into rows of a warp's 256 elements, whose loads run ahead of the draws (16384 x
+  // 1024 bf16: 27 us against 34 by chunks; fp32, with twice the traffic for each draw, gains nothing).
+  const int64_t n = s.rows * s.dim;
+  if (a.vector && full == 8 && s.vec == 8 && n % 256 == 0 && n / 256 < 0x7fffffffLL - (1 << 20)) {
+    NormFwdArgs f{};
+    f.z = z; f.y = y; f.sum = out;
+    f.zs = f.ys = f.ss = f.os = a.os;
+    f.dim = 256; f.in_place = a.in_place; f.drop = a.drop;
+    const int64_t shape1[3] = {1, 1, n / 256};
+    f.map = RowMap::make(shape1, n / 256);
+    f.drop.m[0] = f.drop.m[1] = 0;
+    f.drop.m[2] = 256;
+    return finish(launch_dropout_rows(f, y_dtype, out_dtype, 8, static_cast<cudaStream_t>(stream)), what);
+  }
   return finish(launch_dropout_add(a, z_dtype, y_dtype, out_dtype, s.vec, static_cast<cudaStream_t>(stream)), what);
 }
 
