@@ -720,12 +720,12 @@ struct Split {
 // What a kernel needs to be known for its launches, asked for once per device.
 struct KernelInfo {
   std::mutex mu;
-  int regs[64] = {0};
+  int regs[64] = {0}, own[64] = {0};  // registers of a thread, static shared memory of a CTA
   // CTAs of a launch that fit on an SM at once
   template <class Kernel>
   cudaError_t fit(Kernel kernel, int threads, size_t smem, int* ctas) {
-    constexpr int kSmem = 227 * 1024, kReserved = 1024;  // of an SM; a CTA's own share beside its dynamic one
-    int dev = 0, r = 0, fixed = 2048;
+    constexpr int kSmem = 227 * 1024, kReserved = 1024;  // of an SM; of a CTA, beside what it asks for
+    int dev = 0, r = 0, fixed = 0;
     if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     {
@@ -738,8 +738,10 @@ struct KernelInfo {
             e != cudaSuccess)
           return e;
         regs[dev] = f.numRegs;
+        own[dev] = (int)f.sharedSizeBytes;
       }
       r = regs[dev];
+      fixed = own[dev];
     }
     const int warps = threads / 32;
     int n = 65536 / ((r + 7) / 8 * 8 * 32 * warps);

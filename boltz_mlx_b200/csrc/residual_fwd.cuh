@@ -1,8 +1,13 @@
-// LayerNorm forward, alone or behind dropout + residual add (residual.cuh has the formulas).
+// LayerNorm forward, alone or behind dropout + residual add, and the add without the norm (residual.cuh has the formulas).
 //
-// Bound by HBM: one read of every input and one write of every output.  A persistent grid of row groups; a
-// group's next batches of R rows are on their way into shared memory (residual.cuh) while it works on one.
-// A row's values stay in registers through both statistics passes (mean, then centred squares).
+// Bound by HBM: one read of every input and one write of every output.  A group's next batches of R rows are on their way
+// into shared memory (residual.cuh) while it works on one: with one load in flight for each lane instead, 121 us for 2^20
+// rows of 128 bf16, so 84 us.  A row's values stay in registers through both statistics passes (mean, then centred
+// squares), as pairs, of which one instruction handles two.
+// 2^20 rows of 128: fp32 -> bf16 119 us (1.02 of the copy rate), read transposed 129 us, bf16 84 us, fp32 163 us; with the add
+// and one draw per row 262 us, less than a pass that reads every update needs (286); with a draw per element 327 us: a
+// draw is 20 multiplications of 32 x 32 bits for four elements, at a quarter of the rate of others.
+// 8192 rows of 4096 bf16: 28 us (0.73), of which about 5 are the launch, the parameters and the first rows' way.
 #pragma once
 #include "residual.cuh"
 

@@ -417,7 +417,7 @@ Tensor dropout_add(const Tensor& z, const Tensor& y, double p, uint64_t seed, ui
   if (!inplace) return rec ? DropoutAddFn::apply(opt(z), y, d) : add_forward(z, y, d, z.scalar_type(), Tensor());
   if (z.numel() == 0) return z;
   add_forward(z, y, d, z.scalar_type(), z);
-  z.unsafeGetTensorImpl()->bump_version();
+  if (!z.is_inference()) z.unsafeGetTensorImpl()->bump_version();
   return z;
 }
 

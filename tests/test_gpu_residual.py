@@ -4,7 +4,7 @@
 Tolerances, element by element, from the kernels' arithmetic.  u = 2^-24 is the half step of fp32, U that of
 the output's type.  A row sum has at most K = 16 + 9 + 2 additions on any value's way (16 in a lane, 9 levels
 over 512 lanes) and a multiplication by fp32(1 / dim) (2 u), so with A = max |x| of the row
-  |d mean| <= (K + 2) u A
+  |d mean| <= (K + 3) u A          (one more for the backward pass, which multiplies mean by rstd first)
   |d xh|   <= rstd (|d mean| + u (|x - mean| + A u)) + |xh| e_r,   e_r = relative error of rstd
   e_r      <= ((K + 6) u + 2 |d mean| rstd) / 2 + 4 u       (squares, sum, scaling, eps; rsqrt within 2 ulp = 4 u)
   |d h|    <= |w| |d xh| + 2 u (|w xh| + |b|) + U |h|
@@ -70,7 +70,7 @@ class Row:
         self.b = f64(b) if b is not None else np.zeros(self.x.shape[-1])
         self.h, self.xh, self.rstd = layer_norm_ref(self.x, self.w, self.b, eps)
         A = np.abs(self.x).max(-1, keepdims=True)
-        dmean = (K + 2) * u32 * A
+        dmean = (K + 3) * u32 * A
         self.er = ((K + 6) * u32 + 2 * dmean * self.rstd) / 2 + 4 * u32
         self.dxh = self.rstd * (dmean + u32 * (np.abs(self.xh) / self.rstd + A * u32)) + np.abs(self.xh) * self.er
 
@@ -183,6 +183,33 @@ def test_layer_norm_many_rows(dim):
             close(got[2], rw, tw, F, "dw")
             close(got[3], rb, tb, F, "db")
         assert all(torch.equal(p, q) for p, q in zip(first, got))
+
+
+@pytest.mark.parametrize("dim,rows", [(8, 1700001), (32, 1700001), (64, 900000), (128, 700001), (136, 300001)])
+def test_layer_norm_column_sums_of_many_rows(dim, rows):
+    """Every CTA's partial row has its place: the column sums of so many rows that the work is shared out twice.  A
+    lane adds up at most 4 rows of 32 batches before the joins: Q = 300."""
+    x, dh = normal((rows, dim), B, 1, 0.3), normal((rows, dim), B, 2)
+    w, b = normal((dim,), F, 3, 1.0, 0.2).requires_grad_(), torch.zeros(dim, device="cuda").requires_grad_()
+    dw, db = torch.autograd.grad(layer_norm(x, w, b), (w, b), dh)
+    xd, d = x.double(), dh.double()
+    c = xd - xd.mean(-1, keepdim=True)
+    rstd = (c.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    xh = c * rstd
+    dxh = 1.05 * ((K + 3) * u32 * xd.abs().amax(-1, keepdim=True) * rstd * (1 + xh.abs()) + (K + 14) * u32 * xh.abs())
+    tw = (d.abs() * dxh).sum(0) + 300 * u32 * (d * xh).abs().sum(0)
+    assert ((dw.double() - (d * xh).sum(0)).abs() <= tw).all()
+    assert ((db.double() - d.sum(0)).abs() <= 300 * u32 * d.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("tp", [H, B])
+def test_layer_norm_16_bit_parameters_over_many_ctas(tp):
+    x, dh = normal((3001, 96), F, 1), normal((3001, 96), F, 2)
+    w, b = normal((96,), tp, 3, 1.0, 0.2).requires_grad_(), normal((96,), tp, 4).requires_grad_()
+    (_, rw, rb), (_, tw, tb) = Row(x, w, b).grads(dh)
+    dw, db = torch.autograd.grad(layer_norm(x, w, b), (w, b), dh)
+    close(dw, rw, tw, tp, "dw")
+    close(db, rb, tb, tp, "db")
 
 
 @pytest.mark.parametrize("tp", [F, H, B])
@@ -509,6 +536,18 @@ def test_fused_refusals():
 
 
 # ---- autograd, graphs, streams -----------------------------------------------------------------------------
+def test_inference_mode():
+    z, y, w = normal((4, 8), F, 1), normal((4, 8), F, 2), normal((8,), F, 3).requires_grad_()
+    want = dropout_add(z, y, 0.5, 1)
+    with torch.inference_mode():
+        h = layer_norm(z, w)
+        zi = z + 0.0
+        assert dropout_add(zi, y, 0.5, 1, inplace=True) is zi and torch.equal(zi, want)
+        s, _ = dropout_add_layer_norm(z, y, w, None, 0.5, 1)
+        assert torch.equal(s, want)
+    assert torch.equal(h, layer_norm(z, w).detach())
+
+
 def test_second_derivatives_are_refused():
     x = normal((4, 8), F, 1).requires_grad_()
     d, = torch.autograd.grad(layer_norm(x).square().sum(), x, create_graph=True)
