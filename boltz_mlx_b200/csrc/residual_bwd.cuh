@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
   copy_wait<0>();
 
   if (!a.partial) return;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may take its places and wait
   // groups of one warp first (they own the same channels), then all groups through shared memory
 #pragma unroll
   for (int o = LPR ? LPR : 32; o < 32; o <<= 1) {
@@ -264,6 +265,7 @@ __global__ void __cluster_dims__(kJoin, 1, 1) __launch_bounds__(512)
   const int rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x / kJoin * 32 + lane;  // of 2 * dim
   float s = 0.0f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // all partial rows are written
   if (col < 2 * dim) {
 #pragma unroll 8
     for (int i = rank * 16 + warp; i < ctas; i += 16 * kJoin) s += partial[(size_t)i * 2 * dim + col];
@@ -294,11 +296,20 @@ template <class TP>
 cudaError_t launch_join(const NormBwdArgs& a, int ctas, cudaStream_t st) {
   const int blocks = (2 * a.dim + 31) / 32;
   TP *dw = static_cast<TP*>(a.dweight), *db = static_cast<TP*>(a.dbias);
-  if (ctas > 320 && blocks <= 64)
-    norm_bwd_join_kernel<TP, 8><<<blocks * 8, 512, 0, st>>>(a.partial, ctas, a.dim, dw, db);
-  else
-    norm_bwd_join_kernel<TP, 1><<<blocks, 512, 0, st>>>(a.partial, ctas, a.dim, dw, db);
-  return cudaGetLastError();
+  const int size = ctas > 320 && blocks <= 64 ? 8 : 1;
+  // launched while the last CTAs that write partial rows still run (a pass of 48 us becomes one of 47)
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(blocks * size);
+  c.blockDim = dim3(512);
+  c.stream = st;
+  c.attrs = &early;
+  c.numAttrs = 1;
+  const float* partial = a.partial;
+  if (size == 8) return cudaLaunchKernelEx(&c, norm_bwd_join_kernel<TP, 8>, partial, ctas, (int)a.dim, dw, db);
+  return cudaLaunchKernelEx(&c, norm_bwd_join_kernel<TP, 1>, partial, ctas, (int)a.dim, dw, db);
 }
 
 // Three quarters of the batches go to the CTAs that are resident from the start, in equal shares; the rest in
