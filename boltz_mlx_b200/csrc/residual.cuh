@@ -126,22 +126,10 @@ struct Philox {
 __device__ __forceinline__ uint64_t mask_base(const Dropout& d, const RowIndex& i) {
   return (uint64_t)(d.m[0] * i.i0 + d.m[1] * i.i1 + d.m[2] * i.i2);
 }
-// keep bits of positions pos .. pos + VEC - 1 (VEC 4 or 8: pos is a multiple of 4)
-template <int VEC>
-__device__ __forceinline__ uint32_t keep_bits(const Philox& rng, uint64_t pos, uint32_t drop_max) {
-  if constexpr (VEC == 1) {
-    return rng.word(pos) > drop_max ? 1u : 0u;
-  } else {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int j = 0; j < VEC / 4; ++j) {
-      const uint4 w = rng.block((pos >> 2) + j);
-      bits |= ((w.x > drop_max ? 1u : 0u) | (w.y > drop_max ? 2u : 0u) | (w.z > drop_max ? 4u : 0u) |
-               (w.w > drop_max ? 8u : 0u))
-              << (4 * j);
-    }
-    return bits;
-  }
+// keep bits of a block's four positions
+__device__ __forceinline__ uint32_t keep_bits(const Philox& rng, uint64_t block, uint32_t drop_max) {
+  const uint4 w = rng.block(block);
+  return (w.x > drop_max ? 1u : 0u) | (w.y > drop_max ? 2u : 0u) | (w.z > drop_max ? 4u : 0u) | (w.w > drop_max ? 8u : 0u);
 }
 
 // ---- element types --------------------------------------------------------------------------------
@@ -650,7 +638,7 @@ __device__ __forceinline__ void each_kept(const Lanes<VEC, LPR, NCH>& l, const P
 #pragma unroll
     for (int c = 0; c < NCH; c += 3) {
       const uint64_t mine = (pos0 + warp0 + (c + third) * l.width) >> 2;
-      const uint32_t bits = keep_bits<4>(rng, (mine + block) << 2, drop_max);
+      const uint32_t bits = keep_bits(rng, mine + block, drop_max);
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
         if (c + j < NCH) {

@@ -536,6 +536,97 @@ def test_fused_refusals():
 
 
 # ---- autograd, graphs, streams -----------------------------------------------------------------------------
+def test_gradients_of_broadcast_inputs():
+    """A stream or an update that is broadcast takes the sum of its places' gradients: fp32 sums of 30 values, off by at
+    most 30 u of their absolute sum."""
+    z0, y = normal((1, 1, 1, 40), F, 1).requires_grad_(), normal((2, 3, 5, 40), F, 2).requires_grad_()
+    ds, dh, w = normal((2, 3, 5, 40), F, 3), normal((2, 3, 5, 40), F, 4), normal((40,), F, 5, 1.0, 0.2)
+    for a, b in ((z0.expand(2, 3, 5, 40), y), (y, z0.expand(2, 3, 5, 40))):
+        s, h = dropout_add_layer_norm(a, b, w, None, 0.3, 11, share=(1,))
+        d0, dy = torch.autograd.grad((s, h), (z0, y), (ds, dh))
+        full_a, full_b = a.detach().clone().requires_grad_(), b.detach().clone().requires_grad_()
+        s2, h2 = dropout_add_layer_norm(full_a, full_b, w, None, 0.3, 11, share=(1,))
+        assert torch.equal(s, s2) and torch.equal(h, h2)
+        da, db = torch.autograd.grad((s2, h2), (full_a, full_b), (ds, dh))
+        wide, other = (da, db) if a is not y else (db, da)
+        assert torch.equal(dy, other)
+        ref, tol = wide.double().sum((0, 1, 2), keepdim=True), 30 * u32 * wide.double().abs().sum((0, 1, 2), keepdim=True)
+        assert ((d0.double() - ref).abs() <= tol).all()
+
+
+def test_checkpointed_step_draws_the_same_mask():
+    from torch.utils.checkpoint import checkpoint
+
+    z, y = normal((4, 6, 96), F, 1).requires_grad_(), normal((4, 6, 96), F, 2).requires_grad_()
+    w, g = normal((96,), F, 3, 1.0, 0.1).requires_grad_(), normal((4, 6, 96), F, 4)
+
+    def step(z, y, w):
+        s, h = dropout_add_layer_norm(z, y * y, w, None, 0.4, 5, 9)
+        return dropout_add(s, h, 0.4, 5, 10, share=(0,))
+
+    plain = torch.autograd.grad(step(z, y, w), (z, y, w), g)
+    again = torch.autograd.grad(checkpoint(step, z, y, w, use_reentrant=False), (z, y, w), g)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+
+
+def test_backward_twice():
+    x, w = normal((4, 8), F, 1).requires_grad_(), normal((8,), F, 2).requires_grad_()
+    h = layer_norm(x, w)
+    first = torch.autograd.grad(h.sum(), (x, w), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(h.sum(), (x, w))))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(h.sum(), x)
+
+
+def test_two_threads_at_once():
+    import threading
+
+    x, w, g = normal((300, 256), B, 1), normal((256,), F, 2), normal((300, 256), B, 3)
+    errors = []
+
+    def work(k):
+        try:
+            st = torch.cuda.Stream()
+            st.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(st):
+                for _ in range(30):
+                    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+                    s, h = dropout_add_layer_norm(xs, g, ws, None, 0.5, k, 2)
+                    d = torch.autograd.grad(h, (xs, ws), g)
+                    ref = torch.autograd.grad(layer_norm(s.detach().requires_grad_(), ws), ws, g)
+                    st.synchronize()
+                    if not torch.equal(d[1], ref[0]):
+                        errors.append(k)
+        except Exception as e:  # noqa: BLE001 - reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+
+
+def test_backward_beyond_32_bits():
+    """More than 2^32 elements: the last rows' gradients are those of the first, which have the same values."""
+    dim, rows = 4096, (1 << 20) + 3
+    x1, g1 = normal((1, dim), B, 1), normal((1, dim), B, 2)
+    x, g = x1.expand(rows, dim).requires_grad_(), g1.expand(rows, dim)
+    dx, = torch.autograd.grad(layer_norm(x), x, g)
+    (rx, _, _), (tx, _, _) = Row(x1, None, None).grads(g1)
+    close(dx[:1], rx, tx, B, "dx")
+    for row in (1 << 19, 1 << 20, rows - 1):
+        assert torch.equal(dx[row], dx[0])
+    del dx
+    s, h = dropout_add_layer_norm(x.detach(), g, None, None, 0.5, 3, share=(1,))
+    keep = torch.from_numpy(keep_mask((rows, 1), 0.5, 3, 0)).cuda()[:, 0]
+    for row in (0, 1, 2, rows - 3, rows - 2, rows - 1):
+        assert torch.equal(s[row], (x1.float() + 2.0 * g1.float()).to(B)[0] if keep[row] else x1[0])
+    assert torch.equal(h[rows - 1], layer_norm(s[rows - 1]))
+
+
 def test_inference_mode():
     z, y, w = normal((4, 8), F, 1), normal((4, 8), F, 2), normal((8,), F, 3).requires_grad_()
     want = dropout_add(z, y, 0.5, 1)
