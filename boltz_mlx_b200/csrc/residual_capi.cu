@@ -104,6 +104,12 @@ struct Shape {
     *out = s;
     return TRIATTN_OK;
   }
+  // Two names of one tensor: every element has one place.
+  int alias(const char* name, const Strides3& a, const Strides3& b) const {
+    for (int k = 0; k < 3; ++k)
+      if (n[k] > 1 && a.s[k] != b.s[k]) return fail(TRIATTN_EINVAL, what, "%s aliases z with other strides", name);
+    return TRIATTN_OK;
+  }
   // `share`: bit k = axis k (3: the channels) shares one draw
   int dropout(int share, double p, uint64_t seed, uint64_t offset, const uint64_t* state, Dropout* out) const {
     if (!(p >= 0.0 && p <= 1.0)) return fail(TRIATTN_EINVAL, what, "p=%g must lie in [0, 1]", p);
@@ -183,6 +189,7 @@ int triattn_layer_norm(const void* x, int x_dtype, const int64_t* x_strides, con
   NormFwdArgs a{};
   if (int r = s.tensor("x", x, x_dtype, x_strides, &a.zs, false)) return r;
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
+  if (out == x) return fail(TRIATTN_EINVAL, what, "out aliases x");
   a.z = x; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
   a.mean = mean; a.rstd = rstd;
@@ -209,6 +216,8 @@ int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, co
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
   a.z = z; a.y = y; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.in_place = z == out;
+  if (z && a.in_place)
+    if (int r = s.alias("out", a.zs, a.os)) return r;
   // By chunks: one long vector, rows of more than a warp's worth, and draws per channel over dense rows of an odd width
   // (N=700, 129 fp32 channels: 262 us against 396 by rows).  Else by rows: which of them are dropped whole is then known
   // a batch ahead, and what is dropped is not read (N=1024, one draw per row: 218 us against 280 by chunks).
@@ -258,6 +267,9 @@ int triattn_dropout_add_layer_norm(const void* z, int z_dtype, const int64_t* z_
   if (int r = s.tensor("y", y, y_dtype, y_strides, &a.ys, false)) return r;
   if (int r = s.tensor("sum", sum, z_dtype, sum_strides, &a.ss, true)) return r;
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
+  if (sum == z)
+    if (int r = s.alias("sum", a.zs, a.ss)) return r;
+  if (out == z || out == sum) return fail(TRIATTN_EINVAL, what, "out aliases z or sum");
   a.z = z; a.y = y; a.sum = sum; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
   a.mean = mean; a.rstd = rstd;

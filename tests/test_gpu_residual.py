@@ -726,6 +726,10 @@ def test_layer_norm_module():
         ln(x[..., :64])
     ln(x).sum().backward()
     close(ln.bias.grad, np.full(128, 15.0), np.zeros(128), F, "bias gradient")  # fifteen ones: exact
+    for plain in (b200.LayerNorm(128, elementwise_affine=False).cuda(), b200.LayerNorm(128, bias=False).cuda()):
+        assert torch.equal(plain(x), layer_norm(x))
+    half = b200.LayerNorm(128).cuda().bfloat16()
+    assert half(x.bfloat16()).dtype == B and half(x).dtype == F
 
 
 @pytest.mark.parametrize("precision", ["bf16", "fp16"])

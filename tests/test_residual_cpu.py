@@ -180,7 +180,7 @@ def test_in_place_is_refused(L):
 A = 4096  # an address that validation may look at but nothing may touch
 
 
-def _ln(L, x=A, xd=0, xs=None, shape=(1, 2, 3), dim=8, w=A, b=A, pd=0, eps=1e-5, out=A, od=0, os_=None):
+def _ln(L, x=A, xd=0, xs=None, shape=(1, 2, 3), dim=8, w=A, b=A, pd=0, eps=1e-5, out=2 * A, od=0, os_=None):
     return L.triattn_layer_norm(x, xd, xs, I3(*shape) if shape else None, dim, w, b, pd, eps, out, od, os_, None, None, None)
 
 
@@ -196,7 +196,7 @@ def test_layer_norm_entry_refuses(L):
     assert _ln(L, xd=7) == _lib.EUNSUPPORTED and _ln(L, pd=3) == _lib.EUNSUPPORTED
     assert _ln(L, xd=1, od=2) == _lib.EUNSUPPORTED and _ln(L, xd=2, od=0) == _lib.EUNSUPPORTED
     assert _ln(L, eps=-1.0) == _lib.EINVAL and _ln(L, eps=float("nan")) == _lib.EINVAL and _ln(L, eps=float("inf")) == _lib.EINVAL
-    assert _ln(L, xs=I3(0, -8, 8)) == _lib.EINVAL
+    assert _ln(L, xs=I3(0, -8, 8)) == _lib.EINVAL and _ln(L, out=A) == _lib.EINVAL
     # an output whose rows overlap: a stride below dim, zero, or two axes that meet
     assert _ln(L, os_=I3(0, 8, 4)) == _lib.EINVAL and _ln(L, os_=I3(0, 0, 8)) == _lib.EINVAL
     assert _ln(L, os_=I3(0, 16, 8)) == _lib.EINVAL
@@ -206,7 +206,7 @@ def test_layer_norm_entry_refuses(L):
     assert "layer_norm" in L.triattn_last_error_string().decode()
 
 
-def _da(L, z=A, zd=0, y=A, yd=0, shape=(1, 2, 3), dim=8, share=0, p=0.1, state=None, out=A, od=0, zs=None):
+def _da(L, z=A, zd=0, y=A, yd=0, shape=(1, 2, 3), dim=8, share=0, p=0.1, state=None, out=2 * A, od=0, zs=None):
     return L.triattn_dropout_add(z, zd, zs, y, yd, None, I3(*shape), dim, share, p, 1, 0, state, out, od, None, None)
 
 
@@ -219,13 +219,16 @@ def test_dropout_add_entry_refuses(L):
     assert _da(L, z=None, yd=1, od=2) == _lib.EUNSUPPORTED and _da(L, yd=9) == _lib.EUNSUPPORTED
     assert _da(L, dim=(1 << 30) + 1) == _lib.EUNSUPPORTED
     assert _da(L, zs=I3(-1, 8, 8)) == _lib.EINVAL
+    assert _da(L, out=A, zs=I3(64, 32, 16)) == _lib.EINVAL  # in place through other strides
     assert _da(L, shape=(3, 0, 2), y=None, out=None) == _lib.OK
 
 
 def test_fused_entry_refuses(L):
-    def f(zd=0, yd=0, od=0, s=A, y=A, out=A, p=0.1, share=0, dim=8):
+    def f(zd=0, yd=0, od=0, s=2 * A, y=A, out=3 * A, p=0.1, share=0, dim=8, ss=None):
         return L.triattn_dropout_add_layer_norm(A, zd, None, y, yd, None, I3(1, 2, 3), dim, share, p, 1, 0, None, A, A, 0,
-                                                1e-5, s, None, out, od, None, None, None, None)
+                                                1e-5, s, ss, out, od, None, None, None, None)
+
+    assert f(s=A, ss=I3(64, 32, 16)) == _lib.EINVAL and f(out=A) == _lib.EINVAL and f(s=3 * A) == _lib.EINVAL
 
     assert f(s=None) == _lib.EINVAL and f(y=None) == _lib.EINVAL and f(out=None) == _lib.EINVAL
     assert f(p=2.0) == _lib.EINVAL and f(share=99) == _lib.EINVAL and f(dim=9000) == _lib.EUNSUPPORTED
