@@ -627,7 +627,7 @@ __device__ __forceinline__ void each_kept(const Lanes<VEC, LPR, NCH>& l, const P
         f(w.w > drop_max, c * VEC + q + 3);
       }
     }
-  } else if constexpr (NCH < 3) {
+  } else if constexpr (NCH < 3 || (LPR && LPR < 32)) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) f(rng.word(pos0 + l.col(c)) > drop_max, c);
   } else {
@@ -637,6 +637,7 @@ __device__ __forceinline__ void each_kept(const Lanes<VEC, LPR, NCH>& l, const P
     const int warp0 = l.lane - wl;  // first channel of the warp in piece 0
 #pragma unroll
     for (int c = 0; c < NCH; c += 3) {
+      if (c >= NCH - 4 && warp0 + c * l.width >= l.dim) break;  // the row ends before
       const uint64_t mine = (pos0 + warp0 + (c + third) * l.width) >> 2;
       const uint32_t bits = keep_bits(rng, mine + block, drop_max);
 #pragma unroll
@@ -749,7 +750,7 @@ cudaError_t launch_fused_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int
 cudaError_t launch_fused16_bwd(const NormBwdArgs& a, int x_dtype, int y_dtype, int dout_dtype, int vec, cudaStream_t st);
 cudaError_t launch_dropout_add(const DropoutAddArgs& a, int z_dtype, int y_dtype, int out_dtype, int vec,
                                cudaStream_t st);
-// triattn_dropout_add by rows, dim up to 512
+// triattn_dropout_add by rows, dim up to RES_MAX_DIM
 cudaError_t launch_dropout_rows(const NormFwdArgs& a, int y_dtype, int out_dtype, int vec, cudaStream_t st);
 int norm_bwd_max_ctas();  // of a launch: rows of its partial sums
 

@@ -218,12 +218,14 @@ int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, co
   a.in_place = z == out;
   if (z && a.in_place)
     if (int r = s.alias("out", a.zs, a.os)) return r;
-  // By chunks: one long vector, rows of more than a warp's worth, and draws per channel over dense rows of an odd width
-  // (N=700, 129 fp32 channels: 262 us against 396 by rows).  Else by rows: which of them are dropped whole is then known
-  // a batch ahead, and what is dropped is not read (N=1024, one draw per row: 218 us against 280 by chunks).
+  // By chunks: one long vector, rows of more than 8192 channels, and draws per channel over dense rows of an odd width of
+  // up to 128 (2^24 fp32 elements, draws shared along an axis: 13 channels 104 us against 155 by rows, 63 101 against 119;
+  // 258 channels 82 against 56).  Else by rows: which of them are dropped whole is then known a batch ahead, and what is
+  // dropped is not read (N=1024, one draw per row: 218 us against 280 by chunks; 8192 x 4096 bf16: 28 against 55), and the
+  // loads run ahead of the draws (8192 x 4096 bf16, draws shared along an axis: 43 against 70).
   const int full = y_dtype != DT_F32 && out_dtype != DT_F32 ? 8 : 4;
   const bool dense = (!z || a.zs.dense) && a.ys.dense && a.os.dense;
-  if (s.dim <= 512 && !is_vector(a) && !(a.drop.on && a.drop.per_channel && dense && s.vec < full)) {
+  if (s.dim <= RES_MAX_DIM && !is_vector(a) && !(a.drop.on && a.drop.per_channel && dense && s.vec < full && s.dim <= 128)) {
     NormFwdArgs f{};
     f.z = z; f.y = y; f.sum = out;
     f.zs = z ? a.zs : a.os; f.ys = a.ys; f.ss = f.os = a.os;

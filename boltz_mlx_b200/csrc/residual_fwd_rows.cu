@@ -1,4 +1,4 @@
-// Dropout and residual add by rows of up to 512 channels (residual_fwd.cuh without the norm).
+// Dropout and residual add by rows of up to 8192 channels (residual_fwd.cuh without the norm).
 #include "residual_fwd.cuh"
 
 namespace triattn {
@@ -9,20 +9,33 @@ using B = __nv_bfloat16;
 template <class TX, class TY, Does DO>
 static cudaError_t rows(const NormFwdArgs& a, int vec, cudaStream_t st) {
   constexpr int VEC = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
+#define LAUNCH(VEC, LPR, NCH, R, S, WIDTH, THREADS) return fwd_one<TX, TY, TX, VEC, LPR, NCH, R, S, DO, false>(a, WIDTH, THREADS, st)
   if (vec >= VEC) {
     const int C = a.dim / VEC;
-    if (C <= 8) return fwd_one<TX, TY, TX, VEC, 8, 1, 4, 2, DO, false>(a, 8, 256, st);
-    if (C <= 32) return fwd_one<TX, TY, TX, VEC, 32, 1, 4, 2, DO, false>(a, 32, 256, st);
-    if (C <= 64) return fwd_one<TX, TY, TX, VEC, 32, 2, 2, 2, DO, false>(a, 32, 256, st);
+    if (C <= 8) LAUNCH(VEC, 8, 1, 4, 2, 8, 256);
+    if (C <= 32) LAUNCH(VEC, 32, 1, 4, 2, 32, 256);
+    if (C <= 64) LAUNCH(VEC, 32, 2, 2, 2, 32, 256);
     if constexpr (VEC == 4) {
-      if (C <= 96) return fwd_one<TX, TY, TX, VEC, 32, 3, 2, 2, DO, false>(a, 32, 256, st);
-      return fwd_one<TX, TY, TX, VEC, 32, 4, 2, 2, DO, false>(a, 32, 256, st);
+      if (C <= 96) LAUNCH(VEC, 32, 3, 2, 2, 32, 256);
+      if (C <= 128) LAUNCH(VEC, 32, 4, 2, 2, 32, 256);
     }
+    const RowWidth w = row_width<VEC>(C, 256);
+    if constexpr (VEC == 4) {
+      if (w.pieces == 2) LAUNCH(VEC, 0, 2, 1, 3, w.width, w.threads);
+      if (w.pieces == 3) LAUNCH(VEC, 0, 3, 1, 3, w.width, w.threads);
+    }
+    LAUNCH(VEC, 0, 16 / VEC, 1, 3, w.width, w.threads);
   }
-  if (a.dim <= 128) return fwd_one<TX, TY, TX, 1, 32, 4, 2, 2, DO, false>(a, 32, 256, st);
-  if (a.dim <= 256) return fwd_one<TX, TY, TX, 1, 32, 8, 1, 3, DO, false>(a, 32, 256, st);
-  if (a.dim <= 384) return fwd_one<TX, TY, TX, 1, 32, 12, 1, 3, DO, false>(a, 32, 256, st);
-  return fwd_one<TX, TY, TX, 1, 32, 16, 1, 3, DO, false>(a, 32, 256, st);
+  if (a.dim <= 16) LAUNCH(1, 8, 2, 4, 2, 8, 256);
+  if (a.dim <= 32) LAUNCH(1, 8, 4, 2, 2, 8, 256);
+  if (a.dim <= 128) LAUNCH(1, 32, 4, 2, 2, 32, 256);
+  if (a.dim <= 256) LAUNCH(1, 32, 8, 1, 3, 32, 256);
+  if (a.dim <= 384) LAUNCH(1, 32, 12, 1, 3, 32, 256);
+  if (a.dim <= 512) LAUNCH(1, 32, 16, 1, 3, 32, 256);
+  const RowWidth w = row_width<1>(a.dim, 256);
+  if (w.pieces == 12) LAUNCH(1, 0, 12, 1, 3, w.width, w.threads);
+  LAUNCH(1, 0, 16, 1, 3, w.width, w.threads);
+#undef LAUNCH
 }
 
 cudaError_t launch_dropout_rows(const NormFwdArgs& a, int y, int out, int vec, cudaStream_t st) {

@@ -814,3 +814,50 @@ def test_a_chain_of_the_operators_and_its_gradients():
     ref = chain(wide[0], wide[1:4], wide[4:], norm64, fused64)
     for a, r in zip(got, torch.autograd.grad(ref, wide, g.double())):
         assert float((a.double() - r).abs().max()) <= 2e-4 * float(r.abs().max())
+
+
+@pytest.mark.parametrize("dim,rows", [(1, 1700003), (7, 1700003), (13, 1700003), (31, 900001), (63, 900001), (81, 500001)])
+def test_narrow_odd_rows_column_sums(dim, rows):
+    """Several rows to a warp, over more rows than one share of the work: the column sums with the bound of the other widths
+    (a lane adds up at most 4 rows of 32 batches before the joins: 300 roundings)."""
+    test_layer_norm_column_sums_of_many_rows(dim, rows)
+
+
+@pytest.mark.parametrize("tz,to", [(F, B), (H, H)])
+@pytest.mark.parametrize("dim", [1, 6, 8, 13, 16, 17, 31, 47, 63, 65])
+def test_narrow_rows_to_the_last(dim, tz, to):
+    """Warps and CTAs that the rows do not fill: every row's result and gradients, and nothing behind the last row."""
+    for rows in (1, 3, 31, 32, 33, 1023, 4099):
+        both = normal((2, rows + 2, dim), tz, rows)
+        y, ds, dh = normal((rows, dim), tz, 5), normal((rows, dim), tz, 6), normal((rows, dim), to, 7)
+        z = both[0, :rows].clone().requires_grad_()
+        w = normal((dim,), F, 3, 1.0, 0.2).requires_grad_()
+        y.requires_grad_()
+        s, h = dropout_add_layer_norm(z, y, w, None, 0.4, 3, 1, out_dtype=to)
+        ref = rounded(dropout_add_ref(f64(z), f64(y), 0.4, 3, 1, ()), tz)
+        assert torch.equal(s, ref)
+        r = Row(s, w, None)
+        inside(h, r.h, r.tol_h(to), "h")
+        (rz, _, _), (tz_, _, _) = r.grads(dh, ds)
+        dz, dy, dw = torch.autograd.grad((s, h), (z, y, w), (ds, dh))
+        close(dz, rz, tz_, tz, "dz")
+        keep = dropout_add_ref(None, np.ones((rows, dim)), 0.4, 3, 1, ()) != 0
+        assert (dy.double().cpu().numpy()[~keep] == 0).all()
+        out = both[1].clone()
+        before = out.clone()
+        dropout_add(out[:rows], y.detach(), 0.4, 3, 1, share=(0,), inplace=True)
+        assert torch.equal(out[:rows], rounded(dropout_add_ref(f64(before[:rows]), f64(y), 0.4, 3, 1, (0,)), tz))
+        assert torch.equal(out[rows:], before[rows:])
+
+
+@pytest.mark.parametrize("tz,ty", [(F, F), (F, B), (H, H)])
+@pytest.mark.parametrize("share", [(0,), (1, 2), (1,)])
+@pytest.mark.parametrize("dim", [513, 514, 516, 520, 777, 1028, 1996, 2050, 2560, 4100, 4877, 6144, 8184, 8191, 8192, 8193, 8200])
+def test_dropout_wide_rows(tz, ty, share, dim):
+    z, y = normal((2, 5, dim), tz, 1), normal((5, 2, dim), ty, 2).transpose(0, 1)
+    ref = rounded(dropout_add_ref(f64(z), f64(y), 0.4, 3, 1, share), tz)
+    assert torch.equal(dropout_add(z, y, 0.4, 3, 1, share=share), ref)
+    assert torch.equal(dropout_add(z, y.contiguous(), 0.4, 3, 1, share=share), ref)
+    if tz == ty:
+        dropout_add(z, y, 0.4, 3, 1, share=share, inplace=True)
+        assert torch.equal(z, ref)
