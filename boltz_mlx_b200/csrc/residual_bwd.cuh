@@ -401,6 +401,8 @@ cudaError_t bwd_types(const NormBwdArgs& a, int vec, cudaStream_t st) {
   const bool dense = a.xs.dense && a.dos.dense && (!HASY || !a.ds || a.dss.dense);
   constexpr int FULL = sizeof(TX) == 2 && sizeof(TY) == 2 && sizeof(TO) == 2 ? 8 : 4;
   if (vec >= FULL) return dense ? bwd_vec<TX, TY, TO, FULL, HASY, true>(a, st) : bwd_vec<TX, TY, TO, FULL, HASY, false>(a, st);
+  if constexpr (FULL == 8)
+    if (vec == 4) return dense ? bwd_vec<TX, TY, TO, 4, HASY, true>(a, st) : bwd_vec<TX, TY, TO, 4, HASY, false>(a, st);
   return dense ? bwd_vec<TX, TY, TO, 1, HASY, true>(a, st) : bwd_vec<TX, TY, TO, 1, HASY, false>(a, st);
 }
 

@@ -163,6 +163,19 @@ int check_stats(const char* what, const float* mean, const float* rstd) {
   return TRIATTN_OK;
 }
 
+// Rows that leave lanes of the row form idle, which each draw for a piece (draws per channel cost the most).  2^24 elements
+// with draws shared along an axis, by rows / by chunks in us.  Full pieces on under three quarters of a group of 8, 16 or
+// 32 lanes: fp32 8 channels 111 / 37, 40: 47 / 37, 72: 50 / 38, bf16 72: 40 / 37 (and not: fp32 64: 34 / 38, 96: 41 / 38,
+// bf16 96: 34 / 37).  Odd widths up to 128: fp32 13: 155 / 104, 63: 119 / 101 (and not: 258: 56 / 82).  16-bit rows of
+// four-element pieces, which chunks read one by one: bf16 4: 207 / 82 (and not: 12: 71 / 86, 100: 39 / 86).
+bool leaves_lanes_idle(int dim, int vec, int full) {
+  if (dim <= 8) return true;
+  if (vec == 1) return dim <= 128;
+  if (vec < full) return false;
+  const int pieces = dim / full, lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
+  return 4 * pieces < 3 * lanes;
+}
+
 // Every tensor is dense, and every element has a position of its own, the elements' order (or nothing is dropped).
 bool is_vector(const DropoutAddArgs& a) {
   const int64_t m2 = a.dim, m1 = m2 * a.map.n2.d, m0 = m1 * a.map.n1.d;
@@ -218,14 +231,13 @@ int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, co
   a.in_place = z == out;
   if (z && a.in_place)
     if (int r = s.alias("out", a.zs, a.os)) return r;
-  // By chunks: one long vector, rows of more than 8192 channels, and draws per channel over dense rows of an odd width of
-  // up to 128 (2^24 fp32 elements, draws shared along an axis: 13 channels 104 us against 155 by rows, 63 101 against 119;
-  // 258 channels 82 against 56).  Else by rows: which of them are dropped whole is then known a batch ahead, and what is
-  // dropped is not read (N=1024, one draw per row: 218 us against 280 by chunks; 8192 x 4096 bf16: 28 against 55), and the
-  // loads run ahead of the draws (8192 x 4096 bf16, draws shared along an axis: 43 against 70).
+  // By chunks: one long vector, rows of more than 8192 channels, and what leaves_lanes_idle names.  Else by rows: which of
+  // them are dropped whole is then known a batch ahead, and what is dropped is not read (N=1024, one draw per row: 218 us
+  // against 280 by chunks; 8192 x 4096 bf16: 28 against 55), and the loads run ahead of the draws (8192 x 4096 bf16, draws
+  // shared along an axis: 43 against 70).
   const int full = y_dtype != DT_F32 && out_dtype != DT_F32 ? 8 : 4;
   const bool dense = (!z || a.zs.dense) && a.ys.dense && a.os.dense;
-  if (s.dim <= RES_MAX_DIM && !is_vector(a) && !(a.drop.on && a.drop.per_channel && dense && s.vec < full && s.dim <= 128)) {
+  if (s.dim <= RES_MAX_DIM && !is_vector(a) && !(a.drop.on && a.drop.per_channel && dense && leaves_lanes_idle(s.dim, s.vec, full))) {
     NormFwdArgs f{};
     f.z = z; f.y = y; f.sum = out;
     f.zs = z ? a.zs : a.os; f.ys = a.ys; f.ss = f.os = a.os;

@@ -816,7 +816,8 @@ def test_a_chain_of_the_operators_and_its_gradients():
         assert float((a.double() - r).abs().max()) <= 2e-4 * float(r.abs().max())
 
 
-@pytest.mark.parametrize("dim,rows", [(1, 1700003), (7, 1700003), (13, 1700003), (31, 900001), (63, 900001), (81, 500001)])
+@pytest.mark.parametrize("dim,rows", [(1, 1700003), (4, 1700003), (7, 1700003), (13, 1700003), (20, 900001), (31, 900001), (63, 900001),
+                                      (81, 500001), (100, 400001), (420, 100001)])
 def test_narrow_odd_rows_column_sums(dim, rows):
     """Several rows to a warp, over more rows than one share of the work: the column sums with the bound of the other widths
     (a lane adds up at most 4 rows of 32 batches before the joins: 300 roundings)."""
