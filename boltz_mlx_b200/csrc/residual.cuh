@@ -627,9 +627,29 @@ __device__ __forceinline__ void each_kept(const Lanes<VEC, LPR, NCH>& l, const P
         f(w.w > drop_max, c * VEC + q + 3);
       }
     }
-  } else if constexpr (NCH < 3 || (LPR && LPR < 32)) {
+  } else if constexpr (LPR && NCH > 1) {
+    // A row's channels are next to one another: lane i draws block i of four positions, LPR blocks at a time, and every
+    // lane fetches its bits.  The row may begin inside a block, so that the last piece of four reaches one block further:
+    // the first lane's of the next round.  (Every lane of a warp takes part.)
+    const uint64_t block = (pos0 >> 2) + l.lane;
+    const uint32_t at = ((uint32_t)pos0 & 3) + l.lane;
+    uint32_t bits = keep_bits(rng, block, drop_max);
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) f(rng.word(pos0 + l.col(c)) > drop_max, c);
+    for (int n = 0; n < NCH; n += 4) {
+      uint32_t next = 0;
+      if (NCH >= 4 && (n + 4) * LPR < l.dim + 3) next = keep_bits(rng, block + (n / 4 + 1) * LPR, drop_max);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (n + j < NCH) {
+          const uint32_t drawn = j == 3 && l.lane == 0 ? next : bits;
+          const uint32_t from = (at >> 2) + j * (LPR / 4);
+          f(__shfl_sync(0xffffffffu, drawn, from & (LPR - 1), LPR) >> (at & 3) & 1, n + j);
+        }
+      }
+      bits = next;
+    }
+  } else if constexpr (NCH == 1) {
+    f(rng.word(pos0 + l.col(0)) > drop_max, 0);
   } else {
     // The 32 channels of a warp's piece lie in at most 9 blocks of four positions: lanes 0..8, 9..17 and
     // 18..26 draw those of three pieces at a time, and every lane fetches its bit.
