@@ -163,17 +163,20 @@ int check_stats(const char* what, const float* mean, const float* rstd) {
   return TRIATTN_OK;
 }
 
-// Rows that leave lanes of the row form idle, which each draw for a piece (draws per channel cost the most).  2^24 elements
-// with draws shared along an axis, by rows / by chunks in us.  Full pieces on under three quarters of a group of 8, 16 or
-// 32 lanes: fp32 8 channels 111 / 37, 40: 47 / 37, 72: 50 / 38, bf16 72: 40 / 37 (and not: fp32 64: 34 / 38, 96: 41 / 38,
-// bf16 96: 34 / 37).  Odd widths up to 128: fp32 13: 155 / 104, 63: 119 / 101 (and not: 258: 56 / 82).  16-bit rows of
-// four-element pieces, which chunks read one by one: bf16 4: 207 / 82 (and not: 12: 71 / 86, 100: 39 / 86).
+// Narrow rows that leave over a quarter of the row form's lanes idle, which draw all the same (draws per channel cost the
+// most).  2^24 elements with draws shared along an axis, by rows / by chunks in us.  Whole pieces on lanes for 8, 16 or 32:
+// fp32 8 channels 111 / 37, 40: 47 / 37, 72: 50 / 38, bf16 72: 40 / 37 (and not: fp32 64: 34 / 38, 96: 41 / 38, bf16 96:
+// 34 / 37).  Odd widths on lanes for 32, 64 or 128 channels: fp32 13: 135 / 104, 38: 102 / 83, 66: 115 / 83 (and not: 27:
+// 76 / 104, 55: 72 / 101, 107: 75 / 95).  16-bit rows of four-element pieces, which chunks read one by one: bf16 4: 207 / 82
+// (and not: 12: 71 / 86, 100: 39 / 86).
 bool leaves_lanes_idle(int dim, int vec, int full) {
   if (dim <= 8) return true;
-  if (vec == 1) return dim <= 128;
-  if (vec < full) return false;
-  const int pieces = dim / full, lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
-  return 4 * pieces < 3 * lanes;
+  if (vec > 1 && vec < full) return false;
+  int held = vec == 1 ? 32 : 8 * full;
+  const int most = vec == 1 ? 128 : 32 * full;
+  if (dim > most) return false;
+  while (held < dim) held *= 2;
+  return 4 * dim < 3 * held;
 }
 
 // Every tensor is dense, and every element has a position of its own, the elements' order (or nothing is dropped).

@@ -34,6 +34,7 @@ static cudaError_t rows(const NormFwdArgs& a, int vec, cudaStream_t st) {
   if (vec >= 4) return pieces<TX, TY, DO, 4>(a, st);
   if (a.dim <= 16) LAUNCH(1, 8, 2, 4, 2, 8, 256);
   if (a.dim <= 32) LAUNCH(1, 8, 4, 2, 2, 8, 256);
+  if (a.dim <= 64) LAUNCH(1, 16, 4, 2, 2, 16, 256);
   if (a.dim <= 128) LAUNCH(1, 32, 4, 2, 2, 32, 256);
   if (a.dim <= 256) LAUNCH(1, 32, 8, 1, 3, 32, 256);
   if (a.dim <= 384) LAUNCH(1, 32, 12, 1, 3, 32, 256);
