@@ -21,6 +21,8 @@ must not change; outside a captured graph autograd checks that).
 Types: an fp32 stream with an fp32 or 16-bit result, or one 16-bit type throughout; statistics and sums are
 fp32.  Tensors may have any strides along the leading axes (a transposed pair tensor is read and written in
 place); the last axis is read densely, else copied.  There is no CPU path.
+
+Gradients are those of reverse mode; an input with a forward-mode tangent is refused.
 """
 
 from __future__ import annotations
