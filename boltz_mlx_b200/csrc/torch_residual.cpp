@@ -3,11 +3,14 @@
 // forward and backward pass through Python functions cost 140 us of host time, several times the kernels'
 // own at the usual sizes.  boltz_mlx_b200/residual.py is the public face and checks the numbers (p, seed,
 // shared axes); what concerns the tensors is checked here.
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <stdexcept>
@@ -58,8 +61,15 @@ void on_gpu(const char* what, const Tensor& x, std::initializer_list<const Tenso
 }
 
 // What PyTorch derives from the operators that it sees, it would derive wrongly from these calls, of which it sees the
-// allocation of the results alone: a dual tensor's tangent would be lost, which counts as zero.
-void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+// allocation of the results alone: a tracer (torch.jit.trace; make_fx, before dispatch as well) would record uninitialised
+// memory, fake tensors have no values to work on (an in-place call would change a real one), and a dual tensor's tangent
+// would be lost, which counts as zero.
+void refuse_derived(const char* what, std::initializer_list<const Tensor*> ts) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  if (torch::jit::tracer::isTracing() || Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY) ||
+      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch))
+    unsupported(std::string(what) + ": tracing");
+  if (Modes::get_mode(c10::impl::TorchDispatchModeKey::FAKE)) unsupported(std::string(what) + ": fake tensors");
   for (const Tensor* t : ts)
     if (t->defined() && t->_fw_grad(0).defined())
       unsupported(std::string(what) + ": forward-mode differentiation (an input has a tangent)");
@@ -293,7 +303,7 @@ struct LayerNormNode : ResidualNode {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(3);
-    no_tangent("layer_norm's backward pass", {&grads[0]});
+    refuse_derived("layer_norm's backward pass", {&grads[0]});
     Gradients g;
     {
       at::AutoGradMode off(false);
@@ -314,7 +324,7 @@ struct DropoutAddNode : ResidualNode {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(2);
-    if (task_should_compute_output(1)) no_tangent("dropout_add's backward pass", {&grads[0]});
+    if (task_should_compute_output(1)) refuse_derived("dropout_add's backward pass", {&grads[0]});
     Tensor dz, dy;
     {
       at::AutoGradMode off(false);
@@ -339,7 +349,7 @@ struct FusedNode : ResidualNode {
     if (!ds.defined() && !dh.defined()) return variable_list(4);
     bool want[4];
     for (int k = 0; k < 4; ++k) want[k] = task_should_compute_output(k);
-    if (dh.defined() || want[1]) no_tangent("dropout_add_layer_norm's backward pass", {&ds, &dh});
+    if (dh.defined() || want[1]) refuse_derived("dropout_add_layer_norm's backward pass", {&ds, &dh});
     Gradients g;
     {
       at::AutoGradMode off(false);
@@ -425,7 +435,7 @@ Tensor layer_norm(const Tensor& x0, const Opt& weight, const Opt& bias, double e
   const at::ScalarType out = out_dtype.value_or(x0.scalar_type());
   code_of(out, "out_dtype");
   check_params(what, w, b, x0.size(-1));
-  no_tangent(what, {&x0, &w, &b});
+  refuse_derived(what, {&x0, &w, &b});
   on_gpu(what, x0, {&w, &b});
   const Tensor x = x0.scalar_type() != at::kFloat && out != x0.scalar_type() ? x0.to(at::kFloat) : x0;  // exact
   if (records({&x, &w, &b})) return norm_recorded(x, w, b, eps, out);
@@ -445,7 +455,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
   check_dim("dropout", x, 1 << 30);
   code_of(x, "x");
   const Draw d = draw_of("dropout", x, p, seed, offset, state, share);
-  no_tangent("dropout", {&x});
+  refuse_derived("dropout", {&x});
   on_gpu("dropout", x, {});
   if (records({&x})) return add_recorded(Tensor(), x, d);
   return add_forward(Tensor(), x, d, x.scalar_type(), Tensor());
@@ -465,7 +475,7 @@ Tensor dropout_add(const Tensor& z, const Tensor& y, double p, uint64_t seed, ui
   check_pair(what, z, y);
   check_dim(what, z, 1 << 30);
   const Draw d = draw_of(what, z, p, seed, offset, state, share);
-  no_tangent(what, {&z, &y});
+  refuse_derived(what, {&z, &y});
   const bool rec = records({&z, &y});
   if (inplace && z.numel()) {
     if (rec) throw std::runtime_error("dropout_add: inplace=True keeps no gradients (use torch.no_grad or detach)");
@@ -497,7 +507,7 @@ std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& z, const Tensor&
   if (trans && z.dim() != 4) value_error(std::string(what) + ": trans_out needs [B, I, J, C], got " + str(z.sizes()));
   check_params(what, w, b, z.size(-1));
   const Draw d = draw_of(what, z, p, seed, offset, state, share);
-  no_tangent(what, {&z, &y0, &w, &b});
+  refuse_derived(what, {&z, &y0, &w, &b});
   on_gpu(what, z, {&y0, &w, &b});
   const Tensor y = y0.scalar_type() != z.scalar_type() && y0.scalar_type() != out ? y0.to(at::kFloat) : y0;  // exact
   if (records({&z, &y, &w, &b})) return fused_recorded(z, y, w, b, eps, d, out, trans);

@@ -22,7 +22,8 @@ Types: an fp32 stream with an fp32 or 16-bit result, or one 16-bit type througho
 fp32.  Tensors may have any strides along the leading axes (a transposed pair tensor is read and written in
 place); the last axis is read densely, else copied.  There is no CPU path.
 
-Gradients are those of reverse mode; an input with a forward-mode tangent is refused.
+Gradients are those of reverse mode.  An input with a forward-mode tangent is refused, and so is a call under a tracer
+(torch.jit.trace, make_fx, torch.export) or with fake tensors; torch.compile breaks its graph around a call.
 """
 
 from __future__ import annotations

@@ -3,6 +3,9 @@
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
 
 from boltz_mlx_b200 import _lib, dropout, dropout_add, dropout_add_layer_norm, layer_norm
 from tests.test_gpu_residual import F, normal
@@ -42,3 +45,31 @@ def test_forward_mode_is_refused():
             assert torch.equal(d.primal, y) and torch.equal(d.tangent, torch.ones_like(y))
     for e in ends + through:  # the graphs are still good
         assert torch.isfinite(torch.autograd.grad(e, leaf, y, retain_graph=True)[0]).all()
+
+
+def test_tracing_is_refused():
+    """A traced call, a traced backward pass, and an in-place call on real tensors among fake ones: none is recorded as
+    its uninitialised result, none changes anything."""
+    x, y = normal((3, 40), F, 1), normal((3, 40), F, 2)
+    leaf = x.clone().requires_grad_()
+    calls = [lambda t: layer_norm(t), lambda t: dropout(t, 0.25, 1), lambda t: dropout_add(t, y, 0.25, 1),
+             lambda t: dropout_add_layer_norm(t, y, None, None, 0.25, 1)[1]]
+    for f in calls:
+        h = f(leaf)
+        g, = torch.autograd.grad(h, leaf, y, retain_graph=True)
+        for trace in (lambda f: torch.jit.trace(f, (x,), check_trace=False), lambda f: make_fx(f)(x),
+                      lambda f: make_fx(f, pre_dispatch=True)(x)):
+            with pytest.raises(NotImplementedError, match="tracing"):
+                trace(f)
+        if f is not calls[2]:  # the stream's gradient of dropout_add is the given one
+            with pytest.raises(RuntimeError, match="tracing"):
+                make_fx(lambda g: torch.autograd.grad(h, leaf, g, retain_graph=True)[0])(y)
+        with FlopCounterMode(display=False):
+            assert torch.equal(f(x), h) and torch.equal(torch.autograd.grad(h, leaf, y)[0], g)
+    z = x.clone()
+    with FakeTensorMode():
+        with pytest.raises(NotImplementedError, match="fake"):
+            dropout_add(z, y, 0.25, 1, inplace=True)
+    assert torch.equal(z, x)
+    compiled = torch.compile(lambda t: layer_norm(t * 1.0) + 1.0, backend="eager")
+    assert torch.equal(compiled(x), layer_norm(x) + 1.0)
