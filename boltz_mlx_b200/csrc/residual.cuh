@@ -487,14 +487,16 @@ struct RowIn {
         copy_async_part(dst, reinterpret_cast<const void*>(at), end - at < 16 ? (int)(end - at) : 16);
     }
   }
-  // a row that is not there: zeros
+  // A row that is not there: zeros.  The address, of which nothing is read, is one that a copy may have: of a tensor that
+  // starts anywhere the 16-byte block that holds its start.
   __device__ __forceinline__ void issue_none(int off) const {
     if constexpr (VEC > 1) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) copy_zero<B>(ring32 + off + c * step(), rows.base);
     } else {
+      const void* any = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(rows.base) & ~(uintptr_t)15);
       for (int i = l.lane * 16; i < row_slot<T, VEC, NCH>(l.width, l.dim); i += l.width * 16)
-        copy_zero<16>(ring32 + off + i, rows.base);
+        copy_zero<16>(ring32 + off + i, any);
     }
   }
   __device__ __forceinline__ void read(int off, const T* row, Pair (&x)[L::PAIRS]) const {

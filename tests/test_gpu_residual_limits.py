@@ -8,7 +8,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
 from boltz_mlx_b200 import _lib, dropout, dropout_add, dropout_add_layer_norm, layer_norm
-from tests.test_gpu_residual import F, normal
+from tests.test_gpu_residual import B, F, H, Row, close, inside, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,33 @@ def test_tracing_is_refused():
     assert torch.equal(z, x)
     compiled = torch.compile(lambda t: layer_norm(t * 1.0) + 1.0, backend="eager")
     assert torch.equal(compiled(x), layer_norm(x) + 1.0)
+
+
+@pytest.mark.parametrize("tx,to", [(F, F), (F, B), (H, H)])
+@pytest.mark.parametrize("dim", [8, 13, 128, 333, 1000])
+@pytest.mark.parametrize("rows", [1, 3, 351])
+def test_gradients_of_rows_that_start_anywhere(tx, to, dim, rows):
+    """x and both gradients as views from an odd element on, in rows that fill neither the warps nor the CTAs: what stands
+    for the rows behind the last is zero, and copied from an address that a copy may have."""
+    def at_one(t):
+        r = torch.full((rows * dim + 9,), float("nan"), dtype=t.dtype, device="cuda")
+        r[1:1 + rows * dim] = t.reshape(-1)
+        return r[1:1 + rows * dim].view(rows, dim)
+
+    x, y, w = at_one(normal((rows, dim), tx, 1, 0.5)), at_one(normal((rows, dim), tx, 2)), normal((dim,), F, 3, 1.0, 0.2)
+    ds, dh = at_one(normal((rows, dim), tx, 5)), at_one(normal((rows, dim), to, 6))
+    assert x.data_ptr() % 16 == x.element_size()
+    x.requires_grad_(), w.requires_grad_()
+    h = layer_norm(x, w, out_dtype=to)
+    r = Row(x, w, None)
+    inside(h, r.h, r.tol_h(to), "h")
+    (rx, rw, _), (tx_, tw, _) = r.grads(dh)
+    dx, dw = torch.autograd.grad(h, (x, w), dh)
+    close(dx, rx, tx_, tx, "dx")
+    close(dw, rw, tw, F, "dw")
+    s, h = dropout_add_layer_norm(x, y, w, None, 0.25, 7, out_dtype=to)
+    r = Row(s, w, None)
+    (rx, rw, _), (tx_, tw, _) = r.grads(dh, ds)
+    dx, dw = torch.autograd.grad((s, h), (x, w), (ds, dh))
+    close(dx, rx, tx_, tx, "dz")
+    close(dw, rw, tw, F, "dw of the fused call")
