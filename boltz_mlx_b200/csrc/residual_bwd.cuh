@@ -250,14 +250,22 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
   }
 }
 
+// A value that another kernel wrote while this one was already there: from L2, and not before what stands in front of it.
+__device__ __forceinline__ float ld_written(const float* p) {
+  float v;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // Column sums of the CTAs' partial rows: a cluster of kJoin CTAs for 32 columns, each of its warps with every
 // 16 * kJoin-th row; the cluster's first CTA adds up what the others hold in their shared memory.  One CTA
 // alone needs 15 us for the 2000 partial rows of a long launch, a cluster of eight 3; for the few partial rows
 // of a short launch, or the many columns of long rows, one is enough.
+// The kernel is launched while the rows are still written, so that `partial` is not read-only while it lives: no const
+// __restrict__, and loads that go to L2, behind the wait.
 template <class TP, int kJoin>
 __global__ void __cluster_dims__(kJoin, 1, 1) __launch_bounds__(512)
-    norm_bwd_join_kernel(const float* __restrict__ partial, int ctas, int dim, TP* __restrict__ dweight,
-                         TP* __restrict__ dbias) {
+    norm_bwd_join_kernel(float* partial, int ctas, int dim, TP* dweight, TP* dbias) {
   namespace cg = cooperative_groups;
   __shared__ float part[16][33];
   __shared__ float sum[32];
@@ -268,7 +276,7 @@ __global__ void __cluster_dims__(kJoin, 1, 1) __launch_bounds__(512)
   asm volatile("griddepcontrol.wait;" ::: "memory");  // all partial rows are written
   if (col < 2 * dim) {
 #pragma unroll 8
-    for (int i = rank * 16 + warp; i < ctas; i += 16 * kJoin) s += partial[(size_t)i * 2 * dim + col];
+    for (int i = rank * 16 + warp; i < ctas; i += 16 * kJoin) s += ld_written(partial + (size_t)i * 2 * dim + col);
   }
   part[warp][lane] = s;
   __syncthreads();
@@ -307,7 +315,7 @@ cudaError_t launch_join(const NormBwdArgs& a, int ctas, cudaStream_t st) {
   c.stream = st;
   c.attrs = &early;
   c.numAttrs = 1;
-  const float* partial = a.partial;
+  float* partial = a.partial;
   if (size == 8) return cudaLaunchKernelEx(&c, norm_bwd_join_kernel<TP, 8>, partial, ctas, (int)a.dim, dw, db);
   return cudaLaunchKernelEx(&c, norm_bwd_join_kernel<TP, 1>, partial, ctas, (int)a.dim, dw, db);
 }

@@ -1,5 +1,7 @@
 """GPU: calls of the residual path at the edges of what PyTorch and the C ABI allow."""
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -8,7 +10,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
 from boltz_mlx_b200 import _lib, dropout, dropout_add, dropout_add_layer_norm, layer_norm
-from tests.test_gpu_residual import B, F, H, Row, close, inside, normal
+from tests.test_gpu_residual import B, F, H, Row, close, half, inside, normal, u32
 
 pytestmark = pytest.mark.gpu
 
@@ -103,3 +105,44 @@ def test_gradients_of_rows_that_start_anywhere(tx, to, dim, rows):
     dx, dw = torch.autograd.grad((s, h), (x, w), (ds, dh))
     close(dx, rx, tx_, tx, "dz")
     close(dw, rw, tw, F, "dw of the fused call")
+
+
+C_TYPES = {F: _lib.F32, H: _lib.F16, B: _lib.BF16}
+
+
+def c_backward(x, dh, w, stats, dw, ws):
+    """triattn_layer_norm_backward for dw alone, on the current stream, into a workspace of the caller's."""
+    rows, dim = x.shape
+    _lib.check(_lib.lib().triattn_layer_norm_backward(
+        dh.data_ptr(), C_TYPES[dh.dtype], None, x.data_ptr(), C_TYPES[x.dtype], None, (ctypes.c_int64 * 3)(1, 1, rows), dim,
+        w.data_ptr(), C_TYPES[w.dtype], stats.data_ptr(), stats.data_ptr() + 4 * rows, None, None, 0, 0.0, 0, 0, None, None, None,
+        C_TYPES[x.dtype], dw.data_ptr(), None, ws.data_ptr(), ws.numel(), _lib.stream_handle(x.device)))
+
+
+@pytest.mark.parametrize("rows,dim,t,tp", [(200001, 128, F, F), (200001, 128, B, B), (3001, 64, F, H), (8192, 4096, B, F),
+                                           (777, 1000, H, F)])
+def test_a_workspace_used_by_one_call_behind_another(rows, dim, t, tp):
+    """The kernel that joins the partial sums is there before they are written.  Two calls in turn through one workspace, with
+    nothing between them, give the bits that each gives through one of its own."""
+    w = normal((dim,), tp, 1, 1.0, 0.2)
+    size = _lib.lib().triattn_layer_norm_backward_workspace_bytes(rows, dim)
+    sides = []
+    for seed in (2, 3):
+        x, dh = normal((rows, dim), t, seed, 0.5), normal((rows, dim), t, seed + 10)
+        x64 = x.double()
+        stats = torch.stack([x64.mean(-1), (x64.var(-1, unbiased=False) + 1e-5).rsqrt()]).float().contiguous()
+        own = torch.empty_like(w)
+        c_backward(x, dh, w, stats, own, torch.empty(size, dtype=torch.uint8, device="cuda"))
+        xh = (x64 - stats[0].double()[:, None]) * stats[1].double()[:, None]
+        ref = (dh.double() * xh).sum(0)
+        # as many roundings as the longest way of a value through 200,001 rows of sums has, and those of xh
+        tol = 400 * u32 * (dh.double() * xh).abs().sum(0) + 4 * u32 * (dh.double().abs() * (1 + xh.abs())).sum(0)
+        assert ((own.double() - ref).abs() <= tol + 1.01 * half(tp) * ref.abs()).all()
+        sides.append((x, dh, stats, own))
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    got = [torch.empty((20, dim), dtype=tp, device="cuda") for _ in sides]
+    for k in range(20):
+        for (x, dh, stats, _), out in zip(sides, got):
+            c_backward(x, dh, w, stats, out[k], ws)
+    for (*_, own), out in zip(sides, got):
+        assert torch.equal(out, own.expand(20, dim))
