@@ -1,8 +1,10 @@
 // extern "C" entry points of the residual path (declared in include/triattn.h): argument checks, strides
 // and mask positions, launches on the caller's stream.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <numeric>
 #include <utility>
 
 #include "residual.cuh"
@@ -104,11 +106,50 @@ struct Shape {
     *out = s;
     return TRIATTN_OK;
   }
-  // Two names of one tensor: every element has one place.
-  int alias(const char* name, const Strides3& a, const Strides3& b) const {
-    for (int k = 0; k < 3; ++k)
-      if (n[k] > 1 && a.s[k] != b.s[k]) return fail(TRIATTN_EINVAL, what, "%s aliases z with other strides", name);
-    return TRIATTN_OK;
+  // A tensor that is written and another one of the call: they share no memory, or, where `same` allows it, they are one
+  // tensor under two names (a row is read before it is written, and by the lanes that write it).
+  int apart(const char* written, const void* p, const Strides3& s, int dtype, const char* other, const void* q,
+            const Strides3& t, int other_dtype, bool same) const {
+    const int64_t es = (int64_t)bytes_of(dtype), et = (int64_t)bytes_of(other_dtype);
+    const intptr_t delta = reinterpret_cast<intptr_t>(q) - reinterpret_cast<intptr_t>(p);
+    bool strides = es == et;  // are the same
+    for (int k = 0; k < 3; ++k) strides = strides && (n[k] <= 1 || s.s[k] == t.s[k]);
+    if (same && delta == 0 && strides && dtype == other_dtype) return TRIATTN_OK;
+    if (!meet(s, es, t, et, strides, delta)) return TRIATTN_OK;
+    return fail(TRIATTN_EINVAL, what, "%s overlaps %s%s", written, other, same ? " with other strides, or in part" : "");
+  }
+  // Whether rows of dim elements at strides s and, delta bytes further on, at strides t can have a byte in common.  Exact for
+  // equal strides, and where both lie at multiples of a common pitch; else as their ranges say.
+  bool meet(const Strides3& s, int64_t es, const Strides3& t, int64_t et, bool equal, int64_t delta) const {
+    const int64_t ws = dim * es, wt = dim * et;  // bytes of a row
+    int64_t last_s = 0, last_t = 0, pitch = 0;
+    for (int k = 0; k < 3; ++k) {
+      if (n[k] <= 1) continue;
+      last_s += s.s[k] * es * (n[k] - 1);
+      last_t += t.s[k] * et * (n[k] - 1);
+      pitch = std::gcd(pitch, std::gcd(s.s[k] * es, t.s[k] * et));
+    }
+    if (delta >= last_s + ws || -delta >= last_t + wt) return false;
+    if (pitch > 0) {  // side by side in every pitch
+      const int64_t d = (delta % pitch + pitch) % pitch;
+      if (d >= ws && pitch - d >= wt) return false;
+    }
+    if (!equal) return true;
+    // rows i of one and j of the other lie delta + sum of (j - i) strides apart
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return s.s[a] > s.s[b]; });
+    const auto near = [&](const auto& self, int at, int64_t d) -> bool {
+      if (at == 3) return d < ws && -d < wt;
+      const int k = order[at];
+      if (n[k] <= 1 || s.s[k] == 0) return self(self, at + 1, d);
+      int64_t rest = 0;  // what the smaller strides add at most
+      for (int l = at + 1; l < 3; ++l) rest += n[order[l]] > 1 ? s.s[order[l]] * es * (n[order[l]] - 1) : 0;
+      const int64_t step = s.s[k] * es, around = -d / step, more = (rest + (ws > wt ? ws : wt)) / step + 2;
+      for (int64_t j = around - more; j <= around + more; ++j)
+        if (j > -n[k] && j < n[k] && self(self, at + 1, d + j * step)) return true;
+      return false;
+    };
+    return near(near, 0, delta);
   }
   // `share`: bit k = axis k (3: the channels) shares one draw
   int dropout(int share, double p, uint64_t seed, uint64_t offset, const uint64_t* state, Dropout* out) const {
@@ -205,7 +246,7 @@ int triattn_layer_norm(const void* x, int x_dtype, const int64_t* x_strides, con
   NormFwdArgs a{};
   if (int r = s.tensor("x", x, x_dtype, x_strides, &a.zs, false)) return r;
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
-  if (out == x) return fail(TRIATTN_EINVAL, what, "out aliases x");
+  if (int r = s.apart("out", out, a.os, out_dtype, "x", x, a.zs, x_dtype, false)) return r;
   a.z = x; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
   a.mean = mean; a.rstd = rstd;
@@ -232,8 +273,9 @@ int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, co
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
   a.z = z; a.y = y; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.in_place = z == out;
-  if (z && a.in_place)
-    if (int r = s.alias("out", a.zs, a.os)) return r;
+  if (z)
+    if (int r = s.apart("out", out, a.os, out_dtype, "z", z, a.zs, z_dtype, true)) return r;
+  if (int r = s.apart("out", out, a.os, out_dtype, "y", y, a.ys, y_dtype, true)) return r;
   // By chunks: one long vector, rows of more than 8192 channels, and what leaves_lanes_idle names.  Else by rows: which of
   // them are dropped whole is then known a batch ahead, and what is dropped is not read (N=1024, one draw per row: 218 us
   // against 280 by chunks; 8192 x 4096 bf16: 28 against 55), and the loads run ahead of the draws (8192 x 4096 bf16, draws
@@ -284,9 +326,11 @@ int triattn_dropout_add_layer_norm(const void* z, int z_dtype, const int64_t* z_
   if (int r = s.tensor("y", y, y_dtype, y_strides, &a.ys, false)) return r;
   if (int r = s.tensor("sum", sum, z_dtype, sum_strides, &a.ss, true)) return r;
   if (int r = s.tensor("out", out, out_dtype, out_strides, &a.os, true)) return r;
-  if (sum == z)
-    if (int r = s.alias("sum", a.zs, a.ss)) return r;
-  if (out == z || out == sum) return fail(TRIATTN_EINVAL, what, "out aliases z or sum");
+  if (int r = s.apart("sum", sum, a.ss, z_dtype, "z", z, a.zs, z_dtype, true)) return r;
+  if (int r = s.apart("sum", sum, a.ss, z_dtype, "y", y, a.ys, y_dtype, true)) return r;
+  if (int r = s.apart("out", out, a.os, out_dtype, "z", z, a.zs, z_dtype, false)) return r;
+  if (int r = s.apart("out", out, a.os, out_dtype, "y", y, a.ys, y_dtype, true)) return r;
+  if (int r = s.apart("out", out, a.os, out_dtype, "sum", sum, a.ss, z_dtype, false)) return r;
   a.z = z; a.y = y; a.sum = sum; a.out = out; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.bias = bias; a.param_dtype = param_dtype; a.eps = eps;
   a.mean = mean; a.rstd = rstd;
@@ -309,6 +353,11 @@ int triattn_layer_norm_backward(const void* dout, int dout_dtype, const int64_t*
   Shape s;
   NormBwdArgs a{};
   Strides3 dense;
+  struct Written {
+    const char* name;
+    const void* p;
+    int dtype;
+  };
   if (int r = s.init(what, shape, dim, RES_MAX_DIM)) return r;
   if (!dy) y_dtype = x_dtype;
   if (int r = check_types(what, x_dtype, y_dtype, dout_dtype)) return r;
@@ -340,6 +389,15 @@ int triattn_layer_norm_backward(const void* dout, int dout_dtype, const int64_t*
     if (int r = s.tensor("dx", dx, x_dtype, nullptr, &dense, true)) return r;
   if (dy)
     if (int r = s.tensor("dy", dy, y_dtype, nullptr, &dense, true)) return r;
+  for (const auto& [name, p, dtype] : {Written{"dx", dx, x_dtype}, Written{"dy", dy, y_dtype}}) {
+    if (!p) continue;
+    if (int r = s.apart(name, p, dense, dtype, "dout", dout, a.dos, dout_dtype, true)) return r;
+    if (int r = s.apart(name, p, dense, dtype, "x", x, a.xs, x_dtype, true)) return r;
+    if (dsum)
+      if (int r = s.apart(name, p, dense, dtype, "dsum", dsum, a.dss, x_dtype, true)) return r;
+  }
+  if (dx && dy)
+    if (int r = s.apart("dx", dx, dense, x_dtype, "dy", dy, dense, y_dtype, false)) return r;
   if (!dx && !dy && !dweight && !dbias) return TRIATTN_OK;
   a.dout = dout; a.x = x; a.ds = dsum; a.map = s.map(); a.dim = s.dim;
   a.weight = weight; a.param_dtype = param_dtype; a.mean = mean; a.rstd = rstd;

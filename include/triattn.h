@@ -310,7 +310,10 @@ TRIATTN_API int triattn_forward_noalloc(const float* z, const float* mask, const
  * only read.  x / z are the residual stream.  Types: stream fp32 with an fp32 or 16-bit result, or one
  * 16-bit type throughout; y in the stream's type or the result's; weight, bias and their gradients in
  * param_dtype.  weight NULL = ones, bias NULL = zeros.  dim up to 8192 (triattn_dropout_add: 2^30), fewer
- * than 2^31 - 2^20 rows; an empty axis makes the call empty.  Statistics and sums are fp32.
+ * than 2^31 - 2^20 rows; an empty axis makes the call empty.  Statistics and sums are fp32.  A tensor that is
+ * written shares no memory with another one of the call, unless it is said below that it may be that tensor: at the
+ * same address, with the same type and strides.  Overlapping ones are refused (of tensors whose strides differ, also
+ * some that interleave without a common pitch).
  *
  * Dropout: element e of the mask tensor (the tensor's shape with size 1 along every axis k whose bit k
  * is set in `share`; bit 3 = the channels) takes word e % 4 of Philox4x32-10 with key = seed and
@@ -322,13 +325,13 @@ TRIATTN_API int triattn_forward_noalloc(const float* z, const float* mask, const
 TRIATTN_API int triattn_layer_norm(const void* x, int x_dtype, const int64_t* x_strides, const int64_t* shape,
                                    int64_t dim, const void* weight, const void* bias, int param_dtype, float eps,
                                    void* out, int out_dtype, const int64_t* out_strides, float* mean, float* rstd,
-                                   void* stream); /* mean, rstd: [rows] for the backward pass, or NULL; out is not x */
-/* out = z + dropout(y) (out in z's type, may alias z with the same strides), or dropout(y) with z NULL */
+                                   void* stream); /* mean, rstd: [rows] for the backward pass, or NULL */
+/* out = z + dropout(y) (out in z's type, may be z or y), or dropout(y) with z NULL */
 TRIATTN_API int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, const void* y, int y_dtype,
                                     const int64_t* y_strides, const int64_t* shape, int64_t dim, int share, double p,
                                     uint64_t seed, uint64_t offset, const uint64_t* rng_state, void* out, int out_dtype,
                                     const int64_t* out_strides, void* stream);
-/* sum = z + dropout(y) in z's type (may alias z with the same strides), out = LayerNorm(sum) (neither) */
+/* sum = z + dropout(y) in z's type (may be z or y), out = LayerNorm(sum) (may be y) */
 TRIATTN_API int triattn_dropout_add_layer_norm(const void* z, int z_dtype, const int64_t* z_strides, const void* y,
                                                int y_dtype, const int64_t* y_strides, const int64_t* shape, int64_t dim,
                                                int share, double p, uint64_t seed, uint64_t offset,
@@ -338,7 +341,7 @@ TRIATTN_API int triattn_dropout_add_layer_norm(const void* z, int z_dtype, const
                                                float* rstd, void* stream);
 /* Gradients of the two LayerNorm calls, from x (= sum), mean and rstd as the forward call left them:
  * dx = dsum + LayerNorm'(dout) (dsum: gradient of sum from elsewhere, or NULL), dy = dropout'(dx),
- * dweight, dbias.  Each of dx, dy (dense), dweight and dbias may be NULL.  The workspace (16-byte
+ * dweight, dbias.  Each of dx, dy (dense; either may be dout, x or dsum), dweight and dbias may be NULL.  The workspace (16-byte
  * aligned, for dweight / dbias only) holds one partial row of column sums per CTA; they are summed in a
  * fixed order, so that the same call gives the same bits. */
 TRIATTN_API size_t triattn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim);

@@ -146,3 +146,59 @@ def test_a_workspace_used_by_one_call_behind_another(rows, dim, t, tp):
             c_backward(x, dh, w, stats, out[k], ws)
     for (*_, own), out in zip(sides, got):
         assert torch.equal(out, own.expand(20, dim))
+
+
+def test_outputs_that_are_inputs():
+    """What the C entries allow: an output at the place of the tensor that it is computed from, and tensors side by side in
+    the rows of one buffer, equal the calls with memory of their own bit for bit."""
+    L, shape, dim, p = _lib.lib(), (2, 5, 7), 136, 0.25
+    i3 = (ctypes.c_int64 * 3)(*shape)
+    stream = _lib.stream_handle(torch.device("cuda"))
+    for t in (F, H):
+        c = C_TYPES[t]
+        z, y, ds, dh = (normal((*shape, dim), t, k, 0.5) for k in range(4))
+        w = normal((dim,), F, 5, 1.0, 0.2)
+
+        def add(z, zs, y, ys, out, os_, share):
+            _lib.check(L.triattn_dropout_add(z, c, zs, y, c, ys, i3, dim, share, p, 5, 0, None, out, c, os_, stream))
+
+        for share in (0, 8, 12, 4):
+            want = torch.empty_like(z)
+            add(z.data_ptr(), None, y.data_ptr(), None, want.data_ptr(), None, share)
+            got = y.clone()  # out is y
+            add(z.data_ptr(), None, got.data_ptr(), None, got.data_ptr(), None, share)
+            assert torch.equal(got, want)
+            side = torch.stack([z, torch.zeros_like(z), y], -2)  # z, out and y side by side
+            q, s = side.data_ptr(), (ctypes.c_int64 * 3)(5 * 7 * 3 * dim, 7 * 3 * dim, 3 * dim)
+            step = dim * z.element_size()
+            add(q, s, q + 2 * step, s, q + step, s, share)
+            assert torch.equal(side[..., 1, :], want) and torch.equal(side[..., 0, :], z) and torch.equal(side[..., 2, :], y)
+
+        def fused(z, y, s, out):
+            st = torch.empty((2, 70), device="cuda")
+            _lib.check(L.triattn_dropout_add_layer_norm(
+                z.data_ptr(), c, None, y.data_ptr(), c, None, i3, dim, 0, p, 5, 0, None, w.data_ptr(), None, _lib.F32, 1e-5,
+                s.data_ptr(), None, out.data_ptr(), c, None, st.data_ptr(), st.data_ptr() + 280, stream))
+            return s, out, st
+
+        s, h, st = fused(z, y, torch.empty_like(z), torch.empty_like(z))
+        for into in ("z", "y"):
+            zc, yc = z.clone(), y.clone()
+            got = fused(zc, yc, zc if into == "z" else yc, torch.empty_like(z))
+            assert all(torch.equal(a, b) for a, b in zip(got, (s, h, st)))
+        zc, yc = z.clone(), y.clone()
+        assert all(torch.equal(a, b) for a, b in zip(fused(zc, yc, zc, yc), (s, h, st)))
+
+        def back(dh, x, ds, dx, dy):
+            ws = torch.empty(L.triattn_layer_norm_backward_workspace_bytes(70, dim), dtype=torch.uint8, device="cuda")
+            dw = torch.empty_like(w)
+            _lib.check(L.triattn_layer_norm_backward(
+                dh.data_ptr(), c, None, x.data_ptr(), c, None, i3, dim, w.data_ptr(), _lib.F32, st.data_ptr(), st.data_ptr() + 280,
+                ds.data_ptr(), None, 0, p, 5, 0, None, dx.data_ptr(), dy.data_ptr(), c, dw.data_ptr(), None, ws.data_ptr(),
+                ws.numel(), stream))
+            return dx, dy, dw
+
+        want = back(dh, s, ds, torch.empty_like(z), torch.empty_like(z))
+        for a, b in ((0, 1), (1, 2), (2, 0)):
+            given = [dh.clone(), s.clone(), ds.clone()]
+            assert all(torch.equal(u, v) for u, v in zip(back(*given, given[a], given[b]), want))

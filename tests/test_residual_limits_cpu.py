@@ -1,5 +1,8 @@
 """CPU: what the residual path refuses because its results would be wrong without a word, and what its build keeps in step."""
 
+import ctypes
+import itertools
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -88,3 +91,86 @@ def test_modes_that_record_nothing_are_no_hindrance():
         for f in _calls(*(torch.zeros(2, 8),) * 2, torch.ones(8), torch.zeros(8)):
             with pytest.raises(RuntimeError, match="CUDA"):
                 f()
+
+
+# ---- tensors that overlap, at the C entries --------------------------------------------------------------
+A = 1 << 20  # addresses that validation may look at but nothing may touch: every call here is refused
+
+
+def _strides(s):
+    return None if s is None else (ctypes.c_int64 * 3)(*s)
+
+
+def _add(shape, dim, z, y, out, dtypes=(0, 0)):
+    """triattn_dropout_add of (address, strides); what it says of them."""
+    L = _lib.lib()
+    rc = L.triattn_dropout_add(z[0], dtypes[0], _strides(z[1]), y[0], dtypes[1], _strides(y[1]), _strides(shape), dim, 0, 0.1, 1, 0,
+                               None, out[0], dtypes[0], _strides(out[1]), None)
+    assert rc == _lib.EINVAL
+    return L.triattn_last_error_string().decode()
+
+
+def _bytes(shape, dim, at, strides, es):
+    strides = strides or (shape[1] * shape[2] * dim, shape[2] * dim, dim)
+    return {at + es * sum(i * s for i, s in zip(row, strides)) + k
+            for row in itertools.product(*map(range, shape)) for k in range(dim * es)}
+
+
+def test_overlaps_are_refused_and_nothing_else():
+    """out against z, byte by byte: y always overlaps out, so that the call is refused, for z where z does."""
+    shape, dim = (2, 3, 2), 4
+    layouts = [None, (48, 16, 8), (100, 30, 10), (8, 16, 4), (24, 4, 12), (8, 16, 48), (64, 16, 8)]
+    n = 0
+    for sz in layouts:
+        for so in layouts:
+            for step in (0, 8, 16, 32, 40, 64, 96, 100, 104, 192, 400, 800, 1200):
+                for at in (A + step, A - step):
+                    said = _add(shape, dim, (at, sz), (A + 4, (0, 0, 0)), (A, so))
+                    apart = not _bytes(shape, dim, at, sz, 4) & _bytes(shape, dim, A, so, 4)
+                    one = step == 0 and sz == so
+                    if apart and said.count("overlaps z"):  # only where the strides differ
+                        assert sz != so, (sz, so, at - A, said)
+                        continue
+                    assert ("out overlaps z" in said) != (apart or one), (sz, so, at - A, said)
+                    assert ("out overlaps y" in said) == (apart or one), (sz, so, at - A, said)
+                    n += apart
+    assert n > 100
+
+
+def test_column_slices_of_one_buffer_do_not_overlap():
+    """z and out side by side in the rows of one buffer, out with the leading axes swapped."""
+    said = _add((3, 5, 7), 8, (A, (560, 112, 16)), (A + 4, (0, 0, 0)), (A + 32, (112, 336, 1680)))
+    assert "out overlaps y" in said
+    said = _add((3, 5, 7), 8, (A, (560, 112, 16)), (A + 4, (0, 0, 0)), (A + 28, (112, 336, 1680)))
+    assert "out overlaps z" in said
+
+
+def test_other_entries_refuse_overlaps():
+    L, i3 = _lib.lib(), _strides((1, 2, 3))  # 6 rows of 8: 192 bytes in fp32
+
+    def norm(x, out, od=0, os_=None):
+        return L.triattn_layer_norm(x, 0, None, i3, 8, None, None, 0, 1e-5, out, od, _strides(os_), None, None, None)
+
+    for out in (A, A + 4, A + 188, A - 188):
+        assert norm(A, out) == _lib.EINVAL, out
+    assert norm(A, A - 92, od=1) == _lib.EINVAL and norm(A, A, os_=(48, 8, 16)) == _lib.EINVAL
+
+    def fused(z=A, y=2 * A, s=3 * A, out=4 * A, ss=None, os_=None, ys=None):
+        return L.triattn_dropout_add_layer_norm(z, 0, None, y, 0, _strides(ys), i3, 8, 0, 0.1, 1, 0, None, None, None, 0, 1e-5, s,
+                                                _strides(ss), out, 0, _strides(os_), None, None, None)
+
+    for kw, name in (({"s": A + 32}, "sum overlaps z"), ({"s": 2 * A, "ss": (48, 8, 16)}, "sum overlaps y"),
+                     ({"s": 2 * A - 32}, "sum overlaps y"), ({"out": A}, "out overlaps z"), ({"out": A + 96}, "out overlaps z"),
+                     ({"out": 2 * A + 32}, "out overlaps y"), ({"out": 2 * A, "os_": (48, 8, 16)}, "out overlaps y"),
+                     ({"out": 3 * A}, "out overlaps sum"), ({"out": 3 * A + 64}, "out overlaps sum"),
+                     ({"s": 2 * A, "ys": (0, 0, 0)}, "sum overlaps y")):
+        assert fused(**kw) == _lib.EINVAL and name in L.triattn_last_error_string().decode(), kw
+
+    def back(dout=A, x=2 * A, ds=3 * A, dx=4 * A, dy=5 * A, xs=None):
+        return L.triattn_layer_norm_backward(dout, 0, None, x, 0, _strides(xs), i3, 8, None, 0, A, A, ds, None, 0, 0.0, 0, 0, None,
+                                             dx, dy, 0, None, None, None, 0, None)
+
+    for kw, name in (({"dx": A + 32}, "dx overlaps dout"), ({"dx": 2 * A, "xs": (48, 8, 16)}, "dx overlaps x"),
+                     ({"dx": 3 * A - 32}, "dx overlaps dsum"), ({"dy": A + 32}, "dy overlaps dout"),
+                     ({"dy": 2 * A + 64}, "dy overlaps x"), ({"dx": 5 * A}, "dx overlaps dy"), ({"dx": 5 * A + 32}, "dx overlaps dy")):
+        assert back(**kw) == _lib.EINVAL and name in L.triattn_last_error_string().decode(), kw
