@@ -50,6 +50,12 @@ class PairDropout(NamedTuple):
     share: Optional[Sequence[int]] = None
 
 
+def forward_only(what: str, z: torch.Tensor) -> None:
+    """The layers have no gradients: a result that would lose those of z without a word is refused."""
+    if torch.is_grad_enabled() and z.requires_grad:
+        raise RuntimeError(f"{what}: forward only, z's gradients would be lost (use torch.no_grad or detach)")
+
+
 # ---- numbers --------------------------------------------------------------------------------------------
 @lru_cache(maxsize=256)
 def _share_bits(share: tuple, ndim: int) -> int:

@@ -29,7 +29,7 @@ import warnings
 
 from . import _lib
 from .layout import workspace_bytes
-from .residual import PairDropout, dropout_add, dropout_add_layer_norm, layer_norm
+from .residual import PairDropout, dropout_add, dropout_add_layer_norm, forward_only, layer_norm
 
 
 @contextlib.contextmanager
@@ -230,7 +230,9 @@ class TriangleAttention(nn.Module):
 
     def norm_input(self, z: torch.Tensor) -> torch.Tensor:
         """This module's LayerNorm of z in its 16-bit type and attention orientation (for the ending node read
-        through the transposed view): the `xn` that forward and f16_addln take."""
+        through the transposed view): the `xn` that forward and f16_addln take.  Forward only, as they are: it keeps
+        no gradients of the norm's parameters, and refuses a z that would lose its own."""
+        forward_only("norm_input", z)
         dtype = _lib.dtype_code(self.precision)
         if dtype == _lib.F32:
             raise _lib.TriAttnUnsupported(_lib.EUNSUPPORTED, "xn belongs to the 16-bit path (precision fp16 or bf16)")
@@ -260,9 +262,12 @@ class TriangleAttention(nn.Module):
         instead of its own LN . w_b dot (attention.py:128-147).  `w_tb` [H, c_in] (the next triangle
         attention's tb_weight16()): also return that module's tri bias, computed in the output kernel's
         epilogue from the rounded 16-bit LayerNorm rows (fp32 sums, one rounding to fp16), as
-        [B, H, Q, K] in ln_out's layout (the reference's PAIRTB, kernels_nax3.py:104-143).  `dropout`: a training
-        step's dropout of the update, drawn in the pass that adds it and norms the sum (no w_tb then)."""
+        [B, H, Q, K] in ln_out's layout (the reference's PAIRTB, kernels_nax3.py:104-143).  `dropout`: the
+        dropout of the update in a training step's passes without gradients, drawn in the pass that adds it and norms
+        the sum (no w_tb then).  Forward only: ln_next's parameters get no gradients, and a z that would lose its own
+        is refused."""
         if dropout is not None:
+            forward_only("f16_addln(dropout=)", z)
             if w_tb is not None:
                 raise _lib.TriAttnUnsupported(_lib.EUNSUPPORTED, "w_tb with dropout")
             y = self._run_fused(z, mask, xn, add_residual=False, keep_t=False, tb=tb)[0]
@@ -341,14 +346,17 @@ class TriangleAttention(nn.Module):
     def forward_residual(self, z: torch.Tensor, mask: Optional[torch.Tensor] = None, *,
                          inplace: bool = False, chunk_size: Optional[int] = None,
                          dropout: Optional[PairDropout] = None) -> torch.Tensor:
-        """z + self(z) in one pass (the pairformer's residual update, pairformer.py:86-87).  `dropout`: a training
-        step's dropout of the update (also in its passes without gradients): z + dropout(self(z))."""
+        """z + self(z) in one pass (the pairformer's residual update, pairformer.py:86-87).  `dropout`: the dropout
+        of the update in a training step's passes without gradients: z + dropout(self(z)).  Forward only: a z that would
+        lose its gradients is refused."""
+        if dropout is not None:
+            forward_only("forward_residual(dropout=)", z)
         zc = z.contiguous()
         own = inplace and zc is z and z.dtype == torch.float32
         if dropout is not None:
             y = self._run(zc, mask, False, None, chunk_size)
             with torch.no_grad():
-                r = dropout_add(zc.detach().float(), y, dropout.p, dropout.seed, dropout.offset,
+                r = dropout_add(zc.float(), y, dropout.p, dropout.seed, dropout.offset,
                                 share=self._draw_axes(dropout), inplace=own)
             return zc if own else r
         return self._run(zc, mask, True, zc if own else None, chunk_size)

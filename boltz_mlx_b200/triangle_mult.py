@@ -22,7 +22,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .residual import PairDropout, dropout_add, dropout_add_layer_norm
+from .residual import PairDropout, dropout_add, dropout_add_layer_norm, forward_only
 from .triangle_attention import Workspace
 
 
@@ -95,14 +95,17 @@ class _TriangleMultiplication(nn.Module):
 
     def forward_residual(self, z: torch.Tensor, mask: Optional[torch.Tensor] = None, *,
                          inplace: bool = False, dropout: Optional[PairDropout] = None) -> torch.Tensor:
-        """z + self(z) in one pass (the pairformer's residual update).  `dropout`: a training step's dropout of
-        the update, one draw per row by default: z + dropout(self(z))."""
+        """z + self(z) in one pass (the pairformer's residual update).  `dropout`: the dropout of the update in a
+        training step's passes without gradients, one draw per row by default: z + dropout(self(z)).  Forward only: a z
+        that would lose its gradients is refused."""
+        if dropout is not None:
+            forward_only("forward_residual(dropout=)", z)
         zc = z.contiguous()
         own = inplace and zc is z and z.dtype == torch.float32
         if dropout is not None:
             y = self._run(zc, mask, False, None)
             with torch.no_grad():
-                r = dropout_add(zc.detach().float(), y, dropout.p, dropout.seed, dropout.offset,
+                r = dropout_add(zc.float(), y, dropout.p, dropout.seed, dropout.offset,
                                 share=(2, 3) if dropout.share is None else dropout.share, inplace=own)
             return zc if own else r
         return self._run(zc, mask, True, zc if own else None)
@@ -115,9 +118,12 @@ class _TriangleMultiplication(nn.Module):
         recomputed from z.  `w_tb` [H, 128] (the next triangle attention's tb_weight16()): also return
         that module's tri bias, computed in the tail kernel's epilogue from the rounded 16-bit LayerNorm
         rows (fp32 sums, one rounding to fp16), as [B, H, N, N] (the reference's PAIRTB,
-        kernels_nax3.py:104-143).  `dropout`: a training step's dropout of the update, drawn in the pass that
-        adds it and norms the sum (no w_tb then)."""
+        kernels_nax3.py:104-143).  `dropout`: the dropout of the update in a training step's passes without
+        gradients, drawn in the pass that adds it and norms the sum (no w_tb then).  Forward only: ln_next's parameters
+        get no gradients, and a z that would lose its own is refused."""
         del xn
+        if dropout is not None:
+            forward_only("f16_addln(dropout=)", z)
         if not z.is_cuda:
             raise RuntimeError("TriangleMultiplication (B200) needs CUDA tensors; there is no CPU path")
         dtype = _lib.dtype_code(self.precision)

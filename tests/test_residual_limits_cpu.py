@@ -93,6 +93,28 @@ def test_modes_that_record_nothing_are_no_hindrance():
                 f()
 
 
+# ---- the layers ----------------------------------------------------------------------------------------------
+def test_layers_refuse_to_lose_gradients():
+    """forward_residual and f16_addln with dropout, and norm_input, are forward only: a z with gradients is refused, and one
+    whose gradients nobody asks for gets as far as without."""
+    d, ln = b200.PairDropout(0.25, 1), torch.nn.LayerNorm(128)
+    calls = []
+    for layer in (b200.TriangleAttention(precision="bf16"), b200.TriangleAttention(starting=False, precision="bf16"),
+                  b200.TriangleMultiplicationOutgoing(128, precision="bf16")):
+        calls += [lambda z, m=layer: m.forward_residual(z, dropout=d), lambda z, m=layer: m.f16_addln(z, None, None, ln, dropout=d),
+                  lambda z, m=layer: m.forward_residual(z, dropout=d, inplace=True)]
+        if hasattr(layer, "norm_input"):
+            calls.append(layer.norm_input)
+    z = torch.zeros(1, 4, 4, 128, requires_grad=True)
+    for f in calls:
+        with pytest.raises(RuntimeError, match="forward only"):
+            f(z)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            f(z.detach())
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            f(z)
+
+
 # ---- tensors that overlap, at the C entries --------------------------------------------------------------
 A = 1 << 20  # addresses that validation may look at but nothing may touch: every call here is refused
 
