@@ -136,11 +136,13 @@ __global__ void __launch_bounds__(LPR ? 256 : 512) norm_bwd_kernel(const NormBwd
     for (int r = 0; r < R; ++r) {
       x.read(s * stage + r * slot_x, VEC == 1 ? px[r] : nullptr, xh[r]);
       dout.read(s * stage + r * slot_o, VEC == 1 ? po[r] : nullptr, g[r]);
-      const Pair q = both(rstd[r]), mq = both(-mean[r] * rstd[r]);
+      const Pair q = both(rstd[r]), m = both(-mean[r]);
       Pair s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
-        xh[r][j] = fma2(xh[r][j], q, mq);  // where there is no channel, dout and the weight are zero
+        // centred before it is scaled, as in the forward pass: mean * rstd would be rounded at the size of a row far from
+        // zero.  Where there is no channel, dout and the weight are zero.
+        xh[r][j] = (xh[r][j] + m) * q;
         dw[j] = fma2(g[r][j], xh[r][j], dw[j]);
         db[j] = db[j] + g[r][j];
         g[r][j] = g[r][j] * w[j];

@@ -202,3 +202,26 @@ def test_outputs_that_are_inputs():
         for a, b in ((0, 1), (1, 2), (2, 0)):
             given = [dh.clone(), s.clone(), ds.clone()]
             assert all(torch.equal(u, v) for u, v in zip(back(*given, given[a], given[b]), want))
+
+
+@pytest.mark.parametrize("start", [0, 1])
+@pytest.mark.parametrize("rows", [1, 8])
+@pytest.mark.parametrize("dim", [64, 128, 1024])
+@pytest.mark.parametrize("t,far", [(F, 12345), (H, 1021)])
+def test_gradients_of_rows_far_from_zero(t, far, dim, rows, start):
+    """Whole numbers around a distant one: sums below 2^24, the mean and x - mean are exact in fp32, so that xh has the error of
+    rstd and one rounding, however far the row is from zero (with |d mean| = 0 in the bounds of these gradients)."""
+    g = torch.Generator().manual_seed(dim)
+    e = torch.randint(1, 4, (rows, dim // 2), generator=g)
+    whole = (torch.stack([e, -e], -1) + far).to(t).reshape(-1)
+    x = torch.cat([whole[:start], whole]).cuda()[start:].view(rows, dim).requires_grad_()
+    w, dh = normal((dim,), F, 3, 1.0, 0.2).requires_grad_(), normal((rows, dim), t, 4)
+    h = layer_norm(x, w)
+    r = Row(x, w, None)
+    r.er = (27 + 6) * u32 / 2 + 4 * u32
+    r.dxh = abs(r.xh) * (r.er + u32)
+    inside(h, r.h, r.tol_h(t), "h")
+    (rx, rw, _), (tx, tw, _) = r.grads(dh)
+    dx, dw = torch.autograd.grad(h, (x, w), dh)
+    close(dw, rw, tw, F, "dw")
+    close(dx, rx, tx, t, "dx")
