@@ -49,14 +49,22 @@ def stale() -> bool:
     return _older(LIB, [CSRC / s for s in SOURCES + HEADERS] + [ROOT / "include" / "triattn.h"])
 
 
-def residual_command() -> list[str]:
-    import torch
+def built_for(torch) -> str:
+    """What the binding is compiled against, as it stands in _residual.so."""
+    return f"built for PyTorch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
 
+
+def residual_stale(torch) -> bool:
+    return (_older(RESIDUAL, [RESIDUAL_SOURCE, ROOT / "include" / "triattn.h"])
+            or built_for(torch).encode() + b"\0" not in RESIDUAL.read_bytes())
+
+
+def residual_command(torch) -> list[str]:
     at = Path(torch.__file__).parent
     cuda = Path(nvcc()).resolve().parents[1] if Path(nvcc()).exists() else Path("/usr/local/cuda")
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_residual",
-            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-I{at / 'include'}",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f'-DRESIDUAL_BUILT_FOR="{built_for(torch)}"', f"-I{at / 'include'}",
             f"-I{at / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{cuda / 'include'}",
             f"-I{sysconfig.get_paths()['include']}", f"-I{ROOT / 'include'}", str(RESIDUAL_SOURCE), "-o", str(RESIDUAL),
             f"-L{at / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10",
@@ -77,8 +85,13 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     if force or stale():
         _run([nvcc(), *NVCC_FLAGS, *(extra or []), "-I", str(ROOT / "include"), "-I", str(CSRC),
               "-o", str(LIB), *[str(CSRC / s) for s in SOURCES]], verbose)
-    if force or _older(RESIDUAL, [RESIDUAL_SOURCE, ROOT / "include" / "triattn.h"]):
-        _run(residual_command(), verbose)
+    try:
+        import torch
+    except ImportError:  # the C library needs none
+        print(f"PyTorch is not installed: {RESIDUAL.name}, its binding, is left out")
+        return LIB
+    if force or residual_stale(torch):
+        _run(residual_command(torch), verbose)
     return LIB
 
 

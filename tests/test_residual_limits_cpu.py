@@ -2,6 +2,7 @@
 
 import ctypes
 import itertools
+import sys
 
 import pytest
 import torch
@@ -11,13 +12,12 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
 import boltz_mlx_b200 as b200
-from boltz_mlx_b200 import _lib
+from boltz_mlx_b200 import _lib, build
 
 
 @pytest.fixture(scope="module", autouse=True)
 def _built():
-    if not (_lib.LIB_PATH.exists() and _lib.RESIDUAL_PATH.exists()):
-        pytest.skip("the library is not built (python -m boltz_mlx_b200.build)")
+    build.build()
 
 
 def _calls(x, y, w, b):
@@ -196,3 +196,24 @@ def test_other_entries_refuse_overlaps():
                      ({"dx": 3 * A - 32}, "dx overlaps dsum"), ({"dy": A + 32}, "dy overlaps dout"),
                      ({"dy": 2 * A + 64}, "dy overlaps x"), ({"dx": 5 * A}, "dx overlaps dy"), ({"dx": 5 * A + 32}, "dx overlaps dy")):
         assert back(**kw) == _lib.EINVAL and name in L.triattn_last_error_string().decode(), kw
+
+
+# ---- the build -------------------------------------------------------------------------------------------------
+def test_the_binding_is_rebuilt_for_another_pytorch(monkeypatch, tmp_path):
+    ran = []
+    monkeypatch.setattr(build, "_run", lambda cmd, verbose: ran.append(cmd[-1]))
+    build.build()
+    assert not ran and _lib.residual().built_for == build.built_for(torch)
+    other = tmp_path / "_residual.so"
+    other.write_bytes(build.RESIDUAL.read_bytes().replace(torch.__version__.encode(), b"0" * len(torch.__version__)))
+    monkeypatch.setattr(build, "RESIDUAL", other)
+    build.build()
+    assert len(ran) == 1
+
+
+def test_the_c_library_builds_without_pytorch(monkeypatch, capsys):
+    ran = []
+    monkeypatch.setattr(build, "_run", lambda cmd, verbose: ran.append(str(build.LIB) in cmd))
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build(force=True) == build.LIB and ran == [True]
+    assert "left out" in capsys.readouterr().out
