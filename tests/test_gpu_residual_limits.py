@@ -2,6 +2,7 @@
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -10,7 +11,8 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils.flop_counter import FlopCounterMode
 
 from boltz_mlx_b200 import _lib, dropout, dropout_add, dropout_add_layer_norm, layer_norm
-from tests.test_gpu_residual import B, F, H, Row, close, half, inside, normal, u32
+from oracle.residual_ref import dropout_add_ref, keep_mask, scale_of
+from tests.test_gpu_residual import B, F, H, Row, close, f64, half, inside, normal, rounded, u32
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +227,76 @@ def test_gradients_of_rows_far_from_zero(t, far, dim, rows, start):
     dx, dw = torch.autograd.grad(h, (x, w), dh)
     close(dw, rw, tw, F, "dw")
     close(dx, rx, tx, t, "dx")
+
+
+# ---- every kernel of the fused backward pass -------------------------------------------------------------------
+def check_fused(z, y, w, b, ds, dh, share, p=0.25, seed=77, offset=5, trans=False):
+    """dropout_add_layer_norm of leaves with these values and strides: results, and all gradients, against 64 bits."""
+    leaves = [t.detach().requires_grad_() for t in (z, y, w, b)]
+    s, h = dropout_add_layer_norm(*leaves, p, seed, offset, share=share, out_dtype=dh.dtype, trans_out=trans)
+    assert torch.equal(s, rounded(dropout_add_ref(f64(z), f64(y), p, seed, offset, share), z.dtype))
+    given = dh.transpose(1, 2) if trans else dh
+    r = Row(s, w, b)
+    inside(h.transpose(1, 2) if trans else h, r.h, r.tol_h(dh.dtype), "h")
+    dz, dy, dw, db = torch.autograd.grad((s, h), leaves, (ds, given))
+    (rz, rw, rb), (tz, tw, tb) = r.grads(dh, ds)
+    close(dz, rz, tz, z.dtype, "dz")
+    keep = keep_mask(z.shape, p, seed, offset, share)
+    ry = np.where(keep, rz * scale_of(p), 0.0)
+    close(dy, ry, np.where(keep, scale_of(p) * tz + u32 * np.abs(ry), 0.0), y.dtype, "dy")
+    close(dw, rw, tw, w.dtype, "dw")
+    close(db, rb, tb, b.dtype, "db")
+
+
+FUSED_TYPES = [(F, F, F), (F, F, H), (F, F, B), (F, H, H), (F, B, B), (H, H, H), (B, B, B)]
+
+
+@pytest.mark.parametrize("tz,ty,to", FUSED_TYPES)
+@pytest.mark.parametrize("dim", [4, 13, 36, 65, 100, 101, 129, 260, 333, 388, 421, 500, 510, 700, 777, 1004, 2049, 2060, 4100, 4877,
+                                 6145, 8184, 8191, 8192])
+def test_fused_gradients_of_every_layout(tz, ty, to, dim):
+    """Rows of whole pieces of eight, of four and of one channel, on some lanes of a warp, a warp and several, with one to all
+    of their pieces there; dense, and with every tensor strided in its own way; draws per element, row, column and channel."""
+    for shape in ((2, 3, 5), (3, 41, 17)) if dim < 400 else ((2, 3, 5),):
+        b, i, j = shape
+        z, y, ds, dh = (normal((*shape, dim), t, k, m) for t, k, m in ((tz, 1, 0.5), (ty, 2, 0.0), (tz, 3, 0.0), (to, 4, 0.0)))
+        w, c = normal((dim,), F, 5, 1.0, 0.2), normal((dim,), F, 6, 0.0, 0.2)
+        for share in ((), (2, 3), (1, 3), (1,)):
+            check_fused(z, y, w, c, ds, dh, share)
+        wide = torch.zeros((b, i, j, dim + 8), dtype=tz, device="cuda")
+        wide[..., 8:] = z
+        turned = torch.empty((b, j, i, dim), dtype=ty, device="cuda").copy_(y.transpose(1, 2)).transpose(1, 2)
+        pad = 4 if dim % 8 else 8
+        padded = torch.zeros((b, i, j + 1, dim + pad), dtype=tz, device="cuda")[:, :, :j, pad:]
+        padded.copy_(ds)
+        last = torch.empty((j, i, b, dim), dtype=to, device="cuda").copy_(dh.permute(2, 1, 0, 3)).permute(2, 1, 0, 3)
+        for share in ((), (1, 3)):
+            check_fused(wide[..., 8:], turned, w, c, padded, last, share)
+            check_fused(z, y, w, c, padded, dh, share)  # the gradient of s alone is strided
+
+
+@pytest.mark.parametrize("tz,ty,to", [(F, F, B), (F, B, B), (H, H, H)])
+@pytest.mark.parametrize("dim", [8, 36, 100, 333, 520, 1000, 2052])
+def test_fused_transposed_result_of_other_widths(tz, ty, to, dim):
+    z, y, ds, dh = (normal((2, 7, 9, dim), t, k) for t, k in ((tz, 1), (ty, 2), (tz, 3), (to, 4)))
+    w, b = normal((dim,), F, 5, 1.0, 0.2), normal((dim,), F, 6, 0.0, 0.2)
+    for share in ((), (1, 3)):
+        check_fused(z, y, w, b, ds, dh, share, trans=True)
+
+
+@pytest.mark.parametrize("tz,ty,to", [(F, F, B), (H, H, H), (F, F, F)])
+@pytest.mark.parametrize("dim", [1, 6, 8, 13, 16, 17, 31, 47, 63, 65])
+def test_fused_gradients_of_narrow_rows_to_the_last(tz, ty, to, dim):
+    """Warps and CTAs that the rows do not fill: the values of dy, and the column sums."""
+    for rows in (1, 3, 31, 32, 33, 1023, 4099):
+        z, y, ds, dh = (normal((rows, dim), t, k) for t, k in ((tz, rows), (ty, 5), (tz, 6), (to, 7)))
+        w, b = normal((dim,), F, 8, 1.0, 0.2), normal((dim,), F, 9, 0.0, 0.2)
+        for share in ((), (0,), (1,)):
+            check_fused(z, y, w, b, ds, dh, share, p=0.4)
+
+
+@pytest.mark.parametrize("tp", [H, B])
+@pytest.mark.parametrize("dim", [13, 128, 1004])
+def test_fused_parameters_in_16_bits(tp, dim):
+    z, y, ds, dh = (normal((3, 7, 11, dim), F, k) for k in range(4))
+    check_fused(z, y, normal((dim,), tp, 5, 1.0, 0.2), normal((dim,), tp, 6), ds, dh.to(B), (2, 3))
