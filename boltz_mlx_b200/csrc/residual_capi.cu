@@ -199,6 +199,7 @@ int check_params(const char* what, const void* w, const void* b, int dtype, floa
 }
 
 int check_stats(const char* what, const float* mean, const float* rstd) {
+  if (!mean != !rstd) return fail(TRIATTN_EINVAL, what, "mean without rstd, or rstd without mean");
   if (reinterpret_cast<uintptr_t>(mean) % 4 || reinterpret_cast<uintptr_t>(rstd) % 4)
     return fail(TRIATTN_EINVAL, what, "mean / rstd are not aligned to their elements");
   return TRIATTN_OK;

@@ -325,7 +325,7 @@ TRIATTN_API int triattn_forward_noalloc(const float* z, const float* mask, const
 TRIATTN_API int triattn_layer_norm(const void* x, int x_dtype, const int64_t* x_strides, const int64_t* shape,
                                    int64_t dim, const void* weight, const void* bias, int param_dtype, float eps,
                                    void* out, int out_dtype, const int64_t* out_strides, float* mean, float* rstd,
-                                   void* stream); /* mean, rstd: [rows] for the backward pass, or NULL */
+                                   void* stream); /* mean, rstd: [rows] for the backward pass, or both NULL */
 /* out = z + dropout(y) (out in z's type, may be z or y), or dropout(y) with z NULL */
 TRIATTN_API int triattn_dropout_add(const void* z, int z_dtype, const int64_t* z_strides, const void* y, int y_dtype,
                                     const int64_t* y_strides, const int64_t* shape, int64_t dim, int share, double p,

@@ -198,6 +198,17 @@ def test_other_entries_refuse_overlaps():
         assert back(**kw) == _lib.EINVAL and name in L.triattn_last_error_string().decode(), kw
 
 
+def test_mean_without_rstd_is_refused():
+    """The kernels write both or neither."""
+    L, i3 = _lib.lib(), _strides((1, 2, 3))
+    for mean, rstd in ((A, None), (None, A)):
+        assert L.triattn_layer_norm(A, 0, None, i3, 8, None, None, 0, 1e-5, 2 * A, 0, None, mean, rstd, None) == _lib.EINVAL
+        assert L.triattn_dropout_add_layer_norm(A, 0, None, 2 * A, 0, None, i3, 8, 0, 0.1, 1, 0, None, None, None, 0, 1e-5, 3 * A, None,
+                                                4 * A, 0, None, mean, rstd, None) == _lib.EINVAL
+        assert L.triattn_layer_norm_backward(A, 0, None, 2 * A, 0, None, i3, 8, None, 0, mean, rstd, None, None, 0, 0.0, 0, 0, None,
+                                             3 * A, None, 0, None, None, None, 0, None) == _lib.EINVAL
+
+
 # ---- the build -------------------------------------------------------------------------------------------------
 def test_the_binding_is_rebuilt_for_another_pytorch(monkeypatch, tmp_path):
     ran = []
