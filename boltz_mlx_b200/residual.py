@@ -77,7 +77,7 @@ def _share_bits(share: tuple, ndim: int) -> int:
 
 
 def _share(share, ndim: int) -> int:
-    return _share_bits(share if type(share) is tuple else tuple(share), ndim) if share else 0
+    return _share_bits(share if type(share) is tuple else tuple(share), ndim) if share is not None else 0
 
 
 def _draw(what: str, p: float, seed: Seed, offset: int, training: bool):

@@ -47,6 +47,19 @@ def test_forward_mode_is_refused():
                 f()
 
 
+def test_a_number_is_no_set_of_axes():
+    """share=0 once counted as no shared axis, and dropped each element by itself."""
+    x = torch.zeros(2, 8)
+    for share in (0, 1):
+        for f in (lambda: b200.dropout(x, 0.1, 1, share=share), lambda: b200.dropout_add(x, x, 0.1, 1, share=share),
+                  lambda: b200.dropout_add_layer_norm(x, x, None, None, 0.1, 1, share=share)):
+            with pytest.raises(TypeError):
+                f()
+    for share in ((), [], None, (0,), [0, 1]):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            b200.dropout(x, 0.1, 1, share=share)
+
+
 TRACERS = {
     "jit": lambda f, x: torch.jit.trace(f, (x,), check_trace=False),
     "fx": lambda f, x: make_fx(f)(x),
