@@ -9,9 +9,10 @@
 // handles, so the two column sums stay in its registers until the CTA has seen its last row; they are then joined in
 // shared memory, written as one partial row per CTA and summed by a second small kernel in the order of the CTAs: no
 // atomics, the same bits on every run.
-// 2^20 rows of 128, fp32 <- bf16: 209 us, 6.4 TB/s (0.97 of the copy rate); bf16: 128 us (0.96); with ds and dy, 768^2 rows:
-// 213 us (0.97).  Rows of 4096 in bf16 (8192 of them): 43 us (0.71): about 19 instructions an element on 16 warps an SM,
-// whose registers hold the column sums, and 10 MB of partial sums.
+// 2^20 rows of 128, fp32 <- bf16: 211 us, 6.4 TB/s (0.97 of the copy rate); bf16: 128 us (0.95); with ds and dy, 768^2 rows:
+// 212 us (0.97).  2^25 bf16 in rows of 1024, 2048, 4096 and 8192: 39, 42, 44 and 47 us (0.78, 0.73, 0.70 and 0.66): latency
+// at 16 warps an SM, whose registers hold the column sums; nothing is full (8192 rows of 4096: DRAM 50 %, issue slots 56 %,
+// multipliers 43 %), and up to 10 MB of partial sums are written and read.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -394,7 +395,10 @@ cudaError_t bwd_vec(const NormBwdArgs& a, cudaStream_t st) {
     if (C <= 384) LAUNCH(32, 12, 1, 3, 32, 256);
     if (C <= 512) LAUNCH(32, 16, 1, 3, 32, 256);
   }
-  // long rows: one CTA of 512 threads on an SM leaves half the partial sums that two of 256 do
+  // Long rows: one CTA of 512 threads on an SM leaves half the partial sums that two of 256 do.  2^25 elements in rows of
+  // 2560, 4096 and 8192, 512 against 256: bf16 42.3, 44.0 and 46.5 us against 46.7, 45.1 and 46.5, fp32 70.3, 72.5 and 73.7
+  // against 74.5, 74.6 and 73.8; of 1024, 1536 and 2048: bf16 44.9, 40.1 and 40.6 against 39.5, 42.1 and 42.1, fp32 68.3, 67.4
+  // and 71.1 against 71.1, 67.3 and 73.0.
   const RowWidth w = row_width<VEC>(C, C * VEC > 2048 ? 512 : 256);
   if constexpr (VEC == 4) {
     if (w.pieces == 2) LAUNCH(0, 2, 1, 2, w.width, w.threads);

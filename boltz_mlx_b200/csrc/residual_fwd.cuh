@@ -5,9 +5,12 @@
 // rows of 128 bf16, so 84 us.  A row's values stay in registers through both statistics passes (mean, then centred
 // squares), as pairs, of which one instruction handles two.
 // 2^20 rows of 128: fp32 -> bf16 119 us (1.02 of the copy rate), read transposed 129 us, bf16 84 us, fp32 163 us; with the add
-// and one draw per row 262 us, less than a pass that reads every update needs (286); with a draw per element 327 us: a
-// draw is 20 multiplications of 32 x 32 bits for four elements, at a quarter of the rate of others.
-// 8192 rows of 4096 bf16: 28 us (0.73), of which about 5 are the launch, the parameters and the first rows' way.
+// and one draw per row 262 us, less than a pass that reads every update needs (286; 266 with the kept ones alone); with a
+// draw per element 327 us: a draw is 20 multiplications of 32 x 32 bits for four elements, at a quarter of the rate of others.
+// On 16-bit streams they show: 16384 rows of 1024 bf16, dropout and add 27 us (floor 15), the multipliers busy 64 % of the
+// launch, issue slots 56 %, DRAM 31 %; fused, 8198 rows of 1024 fp16, 18 us (floor 10), 53 / 54 / 20 % at 15 warps an SM.
+// 2^25 bf16 in rows of 1024, 2048, 4096, 8192: 24, 25, 27, 30 us (0.84, 0.82, 0.75, 0.68), of which about 5 are the launch,
+// the parameters and the first rows' way.
 #pragma once
 #include "residual.cuh"
 
@@ -253,7 +256,9 @@ cudaError_t fwd_one(const NormFwdArgs& a, int width, int threads, cudaStream_t s
   // Many CTAs of few batches: they are handed to the SMs as these come free.  An equal share for every resident
   // CTA leaves the SMs that the memory system serves last working alone at the end (0.82 of the copy rate
   // instead of 0.98 at 2^20 rows of 128 fp32).  A CTA has to load weight and bias, though, so that long rows
-  // want more batches, in 16 bits (half the traffic a row) most (0.70 instead of 0.62 at 8192 rows of 4096).
+  // want more batches, in 16 bits (half the traffic a row) most.  2^25 elements in rows of 1024, 2048, 4096 and 8192, 16
+  // batches a CTA against 4: bf16 24.3, 24.8, 26.8 and 29.7 us against 27.2, 27.7, 30.2 and 34.5; fp32 49.0, 50.2, 51.4 and
+  // 52.8 against 43.9, 44.3, 45.1 and 46.8.
   const uint32_t per = groups * R, batches = (a.map.rows + per - 1) / per;
   const uint32_t resident = (uint32_t)(device_sm_count() * fit);
   uint32_t few = (batches + resident - 1) / resident;
