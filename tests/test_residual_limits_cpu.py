@@ -89,6 +89,28 @@ def test_tracing_is_refused(tracer):
         b200.layer_norm(y)
 
 
+@torch.library.custom_op("residual_limits::norm", mutates_args=())
+def _registered(x: torch.Tensor) -> torch.Tensor:
+    return b200.layer_norm(x)
+
+
+@_registered.register_fake
+def _(x):
+    return torch.empty_like(x)
+
+
+@pytest.mark.parametrize("tracer", list(TRACERS))
+def test_a_registered_operator_is_no_hindrance(tracer):
+    """A program may register a call as an operator of its own: a tracer records that, and the call inside is not traced."""
+    trace = lambda: TRACERS[tracer](lambda x: torch.ops.residual_limits.norm(x), torch.zeros(2, 8))  # noqa: E731
+    if tracer in ("fx of fake tensors", "export"):
+        graph = trace()
+        assert "residual_limits.norm" in str(getattr(graph, "graph_module", graph).graph)
+    else:  # these run what they record
+        with pytest.raises(RuntimeError, match="CUDA"):
+            trace()
+
+
 def test_fake_tensors_are_refused():
     real, w, b = torch.zeros(2, 8), torch.ones(8), torch.zeros(8)
     with FakeTensorMode():
